@@ -38,6 +38,7 @@ Options& options()
 namespace {
 
 constexpr int kMaxDevices = 64;
+constexpr int kSlots = 6;
 constexpr int64_t kTileFlagInts = 1 << 18;   // 1 MiB of per-tile counters per device, shared by the replicated launches in flight
 
 thread_local std::string t_error;
@@ -60,12 +61,13 @@ int fail_cuda(const char* what, cudaError_t e)
 // for host-pointer calls and a scratch buffer for multi-pass kernels.
 struct DeviceState {
     std::mutex mu;
+    std::mutex pool_mu;             // creation of the pool (calls on host pointers hold mu while they allocate from it)
     bool ready = false;
     int num_sms = 0;
     int* status = nullptr;          // device, kStatusWords ints
     int* status_host = nullptr;     // pinned mirror
-    void* slot[4] = { nullptr, nullptr, nullptr, nullptr };   // staging: A/data, B/indices, C/output, bias
-    size_t slot_bytes[4] = { 0, 0, 0, 0 };
+    void* slot[kSlots] = {};        // staging: A/data, B/indices, C/output, bias, scales of A, scales of B
+    size_t slot_bytes[kSlots] = {};
     void* scratch = nullptr;
     size_t scratch_bytes = 0;
     // the scratch buffer is shared by all streams of the device: a launch that uses it on another stream than
@@ -78,6 +80,7 @@ struct DeviceState {
     int64_t tile_flags_cursor = 0;
     cudaStream_t pipe[2] = { nullptr, nullptr };   // staging pipeline of large host-pointer GEMMs
     cudaEvent_t pipe_ready = nullptr;              // B (and bias) have arrived
+    cudaMemPool_t pool = nullptr;                  // stream-ordered temporaries (temp_alloc)
 };
 DeviceState g_dev[kMaxDevices];
 
@@ -156,11 +159,11 @@ int ensure(void** buf, size_t* have, size_t need)
 //          accb_synchronize and does not become this call's result.
 //   what = COLLECT_ALL: accb_synchronize reports whatever is recorded.
 // What is reported is cleared.
-enum { COLLECT_ALL = 0, COLLECT_GEMM = 1, COLLECT_GATHER = 2 };
+enum { COLLECT_ALL = 0, COLLECT_GEMM = 1, COLLECT_GATHER = 2, COLLECT_EMBED = 3 };
 
-int decode_status(const int* w, int what, int id, bool* clear_gemm, bool* clear_gather, std::string* msg)
+int decode_status(const int* w, int what, int id, bool* clear_gemm, bool* clear_gather, bool* clear_embed, std::string* msg)
 {
-    *clear_gemm = *clear_gather = false;
+    *clear_gemm = *clear_gather = *clear_embed = false;
     const bool gemm_failed = w[ST_GEMM_ID] != 0 || w[ST_GEMM_COUNT] != 0;
     const bool gemm_mine = what == COLLECT_ALL || (what == COLLECT_GEMM && w[ST_GEMM_ID] == id);
     if (gemm_failed && gemm_mine) {
@@ -185,6 +188,15 @@ int decode_status(const int* w, int what, int id, bool* clear_gemm, bool* clear_
         *clear_gather = true;
         return ACCB_ERR_INDEX;
     }
+    const bool embed_mine = what == COLLECT_ALL || (what == COLLECT_EMBED && w[ST_EMBED_ID] == id);
+    if (w[ST_EMBED_COUNT] != 0 && embed_mine) {
+        char buf[200];
+        snprintf(buf, sizeof buf, "embedding: %d token id(s) outside the table; their rows were zero-filled or left out of the gradient",
+                 w[ST_EMBED_COUNT]);
+        *msg = buf;
+        *clear_embed = true;
+        return ACCB_ERR_INDEX;
+    }
     return ACCB_OK;
 }
 
@@ -195,15 +207,16 @@ int collect_status(DeviceState& s, cudaStream_t stream, int what = COLLECT_ALL, 
     if (e != cudaSuccess) return fail_cuda("kernel execution", e);
     int w[kStatusWords];
     memcpy(w, s.status_host, sizeof w);
-    bool clear_gemm = false, clear_gather = false;
+    bool clear_gemm = false, clear_gather = false, clear_embed = false;
     std::string msg;
-    const int rc = decode_status(w, what, id, &clear_gemm, &clear_gather, &msg);
+    const int rc = decode_status(w, what, id, &clear_gemm, &clear_gather, &clear_embed, &msg);
     if (rc == ACCB_OK) return ACCB_OK;
     if (clear_gemm) e = cudaMemsetAsync(s.status + ST_GEMM_SITE, 0, 4 * sizeof(int), stream);      // words 1..4
     if (clear_gather && e == cudaSuccess) {
         e = cudaMemsetAsync(s.status + ST_GATHER_COUNT, 0, sizeof(int), stream);
         if (e == cudaSuccess) e = cudaMemsetAsync(s.status + ST_GATHER_ID, 0, sizeof(int), stream);
     }
+    if (clear_embed && e == cudaSuccess) e = cudaMemsetAsync(s.status + ST_EMBED_COUNT, 0, 2 * sizeof(int), stream);   // words 6, 7
     if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
     if (e != cudaSuccess) return fail_cuda("cudaMemsetAsync(status)", e);
     return fail(rc, msg);
@@ -227,6 +240,30 @@ int64_t span_elems(int64_t d0, int64_t d1, const int64_t* st)
 }
 
 }  // namespace
+
+void* temp_alloc(int device, size_t bytes, cudaStream_t stream)
+{
+    // A pool of the library's own, because the device's default pool gives its memory back at every synchronisation and
+    // the next allocation then costs tens of microseconds.
+    DeviceState& s = g_dev[device];
+    {
+        std::lock_guard<std::mutex> lock(s.pool_mu);
+        if (!s.pool) {
+            cudaMemPoolProps props = {};
+            props.allocType = cudaMemAllocationTypePinned;
+            props.location.type = cudaMemLocationTypeDevice;
+            props.location.id = device;
+            if (cudaMemPoolCreate(&s.pool, &props) != cudaSuccess) { (void)cudaGetLastError(); s.pool = nullptr; return nullptr; }
+            uint64_t keep = UINT64_MAX;
+            cudaMemPoolSetAttribute(s.pool, cudaMemPoolAttrReleaseThreshold, &keep);
+        }
+    }
+    void* p = nullptr;
+    if (cudaMallocFromPoolAsync(&p, bytes, s.pool, stream) != cudaSuccess) { (void)cudaGetLastError(); return nullptr; }
+    return p;
+}
+
+void temp_free(void* p, cudaStream_t stream) { if (p) cudaFreeAsync(p, stream); }
 
 int set_error(int code, const char* msg) { return fail(code, msg ? msg : ""); }
 void clear_error() { t_error.clear(); }
@@ -825,6 +862,222 @@ int accb_gather_rank2(const void* data, int64_t d0, int64_t d1, const int64_t* i
     return collect_status(s, stream, COLLECT_GATHER, launch_id);
 }
 
+static bool is_float_type(int t) { return t == ACCB_F32 || t == ACCB_F16 || t == ACCB_BF16; }
+
+// accb_embedding (grad = false: table is read, rows written) and accb_embedding_grad (rows read, table updated)
+static int embedding_entry(const char* fn, bool grad, const accb_embedding_desc* desc, const void* table, const void* ids, const void* rows)
+{
+    t_error.clear();
+    const std::string who = std::string(fn) + ": ";
+    if (!desc) return fail(ACCB_ERR_ARG, who + "null descriptor");
+    const accb_embedding_desc& d = *desc;
+    if (d.tokens < 0 || d.vocab < 0 || d.dim < 0) return fail(ACCB_ERR_ARG, who + "negative dimension");
+    const int64_t lim = ((int64_t)1 << 31) - 1;
+    if (d.tokens >= lim || d.vocab >= lim || d.dim >= lim) return fail(ACCB_ERR_ARG, who + "dimension too large");
+    if (!is_float_type(d.table_type) || !is_float_type(d.rows_type)) return fail(ACCB_ERR_ARG, who + "table and rows are fp32, fp16 or bf16");
+    if (d.id_bytes != 4 && d.id_bytes != 8) return fail(ACCB_ERR_ARG, who + "id_bytes must be 4 or 8");
+    if (d.reserved != 0) return fail(ACCB_ERR_ARG, who + "reserved must be 0");
+    if ((d.vocab > 1 && d.table_stride < d.dim) || (d.tokens > 1 && d.rows_stride < d.dim))
+        return fail(ACCB_ERR_ARG, who + "row strides must be at least dim");
+    if (d.dim > (int64_t)1 << 20) return fail(ACCB_ERR_ARG, who + "dim is at most 2^20");
+    if (d.dim == 0 || (grad ? d.vocab : d.tokens) == 0) return ACCB_OK;
+    if ((d.vocab > 0 && !table) || (d.tokens > 0 && (!ids || !rows))) return fail(ACCB_ERR_ARG, who + "null array pointer");
+
+    DeviceState* sp = nullptr;
+    int dev = 0;
+    int rc = device_state(&sp, &dev);
+    if (rc != ACCB_OK) return rc;
+    DeviceState& s = *sp;
+    EmbeddingLaunch l;
+    l.d = d;
+    l.stream = t_stream;
+    l.status = s.status;
+    l.launch_id = next_launch_id();
+    l.num_sms = s.num_sms;
+    l.device = dev;
+    // an empty side may have any pointer
+    const bool dev_written = is_device_pointer(grad ? table : rows);
+    const bool dev_ids = d.tokens ? is_device_pointer(ids) : dev_written;
+    const bool dev_read = grad ? (d.tokens ? is_device_pointer(rows) : dev_written) : (d.vocab ? is_device_pointer(table) : dev_written);
+    if (dev_ids != dev_written || dev_read != dev_written) return fail(ACCB_ERR_ARG, who + "mix of host and device pointers");
+    const char* err = "";
+    if (dev_written) {
+        l.ids = ids;
+        const int n = grad ? launch_embedding_grad(l, rows, const_cast<void*>(table), &err) : launch_embedding(l, table, const_cast<void*>(rows), &err);
+        return n < 0 ? fail(n, who + err) : ACCB_OK;
+    }
+    std::lock_guard<std::mutex> lock(s.mu);
+    const size_t et = type_bytes(d.table_type), er = type_bytes(d.rows_type);
+    const size_t bytes_table = d.vocab ? ((size_t)(d.vocab - 1) * d.table_stride + d.dim) * et : 0;
+    const size_t bytes_rows = d.tokens ? ((size_t)(d.tokens - 1) * d.rows_stride + d.dim) * er : 0;
+    const size_t bytes_ids = (size_t)d.tokens * d.id_bytes;
+    if ((rc = ensure(&s.slot[0], &s.slot_bytes[0], bytes_table)) != ACCB_OK) return rc;
+    if ((rc = ensure(&s.slot[1], &s.slot_bytes[1], bytes_ids)) != ACCB_OK) return rc;
+    if ((rc = ensure(&s.slot[2], &s.slot_bytes[2], bytes_rows)) != ACCB_OK) return rc;
+    // the written side goes to the device too where it is read or has gaps between its rows, whose bytes come back
+    const bool gaps = grad ? d.table_stride != d.dim : d.rows_stride != d.dim;
+    const bool table_in = bytes_table && (!grad || d.beta != 0.0f || gaps), rows_in = bytes_rows && (grad || gaps);
+    cudaError_t e = cudaSuccess;
+    if (table_in) e = cudaMemcpyAsync(s.slot[0], table, bytes_table, cudaMemcpyHostToDevice, l.stream);
+    if (e == cudaSuccess && bytes_ids) e = cudaMemcpyAsync(s.slot[1], ids, bytes_ids, cudaMemcpyHostToDevice, l.stream);
+    if (e == cudaSuccess && rows_in) e = cudaMemcpyAsync(s.slot[2], rows, bytes_rows, cudaMemcpyHostToDevice, l.stream);
+    if (e != cudaSuccess) return fail_cuda("host to device copy", e);
+    l.ids = s.slot[1];
+    const int n = grad ? launch_embedding_grad(l, s.slot[2], s.slot[0], &err) : launch_embedding(l, s.slot[0], s.slot[2], &err);
+    if (n < 0) return fail(n, who + err);
+    e = grad ? cudaMemcpyAsync(const_cast<void*>(table), s.slot[0], bytes_table, cudaMemcpyDeviceToHost, l.stream)
+             : cudaMemcpyAsync(const_cast<void*>(rows), s.slot[2], bytes_rows, cudaMemcpyDeviceToHost, l.stream);
+    if (e != cudaSuccess) return fail_cuda("device to host copy", e);
+    return collect_status(s, l.stream, COLLECT_EMBED, l.launch_id);
+}
+
+int accb_embedding(const accb_embedding_desc* desc, const void* table, const void* ids, void* rows)
+{
+    return embedding_entry("accb_embedding", false, desc, table, ids, rows);
+}
+
+int accb_embedding_grad(const accb_embedding_desc* desc, const void* rows, const void* ids, void* table)
+{
+    return embedding_entry("accb_embedding_grad", true, desc, table, ids, rows);
+}
+
+static bool is_fp8_type(int t) { return t == ACCB_E4M3 || t == ACCB_E5M2; }
+
+int accb_quantize_fp8(const accb_quantize_fp8_desc* desc, const void* x, void* q, float* scales)
+{
+    t_error.clear();
+    const std::string who = "accb_quantize_fp8: ";
+    if (!desc) return fail(ACCB_ERR_ARG, who + "null descriptor");
+    const accb_quantize_fp8_desc& d = *desc;
+    if (d.rows < 0 || d.cols < 0) return fail(ACCB_ERR_ARG, who + "negative dimension");
+    const int64_t lim = ((int64_t)1 << 31) - 1;
+    if (d.rows >= lim || d.cols >= lim) return fail(ACCB_ERR_ARG, who + "dimension too large");
+    if (!is_float_type(d.x_type)) return fail(ACCB_ERR_ARG, who + "x is fp32, fp16 or bf16");
+    if (!is_fp8_type(d.q_type)) return fail(ACCB_ERR_ARG, who + "q is ACCB_E4M3 or ACCB_E5M2");
+    if (d.block_rows != 1 && d.block_rows != ACCB_FP8_BLOCK) return fail(ACCB_ERR_ARG, who + "block_rows must be 1 or 128");
+    if (d.reserved != 0) return fail(ACCB_ERR_ARG, who + "reserved must be 0");
+    for (int i = 0; i < 2; ++i)
+        if (d.x_stride[i] < 1 || d.scale_stride[i] < 1) return fail(ACCB_ERR_ARG, who + "strides must be positive");
+    if (d.rows > 1 && d.q_stride < d.cols) return fail(ACCB_ERR_ARG, who + "q_stride must be at least cols");
+    if (d.rows == 0 || d.cols == 0) return ACCB_OK;
+    if (!x || !q || !scales) return fail(ACCB_ERR_ARG, who + "null array pointer");
+
+    DeviceState* sp = nullptr;
+    int rc = device_state(&sp, nullptr);
+    if (rc != ACCB_OK) return rc;
+    DeviceState& s = *sp;
+    const bool dx = is_device_pointer(x), dq = is_device_pointer(q), ds = is_device_pointer(scales);
+    if (dx != dq || dx != ds) return fail(ACCB_ERR_ARG, who + "mix of host and device pointers");
+    cudaStream_t stream = t_stream;
+    const char* err = "";
+    if (dx) {
+        const int n = launch_quantize_fp8(d, x, q, scales, stream, &err);
+        return n < 0 ? fail(n, who + err) : ACCB_OK;
+    }
+    std::lock_guard<std::mutex> lock(s.mu);
+    const int64_t srows = (d.rows + d.block_rows - 1) / d.block_rows, scols = (d.cols + ACCB_FP8_BLOCK - 1) / ACCB_FP8_BLOCK;
+    const size_t bytes_x = (size_t)span_elems(d.rows, d.cols, d.x_stride) * type_bytes(d.x_type);
+    const size_t bytes_q = (size_t)(d.rows - 1) * d.q_stride + d.cols;
+    const size_t bytes_s = (size_t)span_elems(srows, scols, d.scale_stride) * 4;
+    if ((rc = ensure(&s.slot[0], &s.slot_bytes[0], bytes_x)) != ACCB_OK) return rc;
+    if ((rc = ensure(&s.slot[2], &s.slot_bytes[2], bytes_q)) != ACCB_OK) return rc;
+    if ((rc = ensure(&s.slot[4], &s.slot_bytes[4], bytes_s)) != ACCB_OK) return rc;
+    cudaError_t e = cudaMemcpyAsync(s.slot[0], x, bytes_x, cudaMemcpyHostToDevice, stream);
+    // outputs with gaps: the copy back covers them, so they must carry the caller's bytes
+    if (e == cudaSuccess && bytes_q != (size_t)(d.rows * d.cols)) e = cudaMemcpyAsync(s.slot[2], q, bytes_q, cudaMemcpyHostToDevice, stream);
+    if (e == cudaSuccess && bytes_s != (size_t)(srows * scols) * 4) e = cudaMemcpyAsync(s.slot[4], scales, bytes_s, cudaMemcpyHostToDevice, stream);
+    if (e != cudaSuccess) return fail_cuda("host to device copy", e);
+    const int n = launch_quantize_fp8(d, s.slot[0], s.slot[2], (float*)s.slot[4], stream, &err);
+    if (n < 0) return fail(n, who + err);
+    e = cudaMemcpyAsync(q, s.slot[2], bytes_q, cudaMemcpyDeviceToHost, stream);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(scales, s.slot[4], bytes_s, cudaMemcpyDeviceToHost, stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    if (e != cudaSuccess) return fail_cuda("device to host copy", e);
+    return ACCB_OK;
+}
+
+// Picks the kernel for one 8-bit GEMM on device pointers.  Returns launches made or a negative ACCB_ERR_*.
+static int dispatch_gemm_fp8(const GemmFp8Launch& g, const char** err)
+{
+    if (g.d.compute == ACCB_COMPUTE_TENSOR && g.d.k > 0) { *err = "no tensor-core kernel takes these operands"; return ACCB_ERR_ARG; }
+    return launch_gemm_fp8_simt(g, err);
+}
+
+int accb_gemm_fp8(const accb_gemm_desc* desc, const accb_fp8_scales* scales, const void* a, const void* b, void* c,
+                  const float* a_scales, const float* b_scales, const float* bias)
+{
+    t_error.clear();
+    const std::string who = "accb_gemm_fp8: ";
+    if (!desc || !scales) return fail(ACCB_ERR_ARG, who + "null descriptor");
+    const accb_gemm_desc& d = *desc;
+    if (d.m < 0 || d.n < 0 || d.k < 0) return fail(ACCB_ERR_ARG, who + "negative dimension");
+    const int64_t lim = (int64_t)1 << 30;
+    if (d.m > lim || d.n > lim || d.k > lim) return fail(ACCB_ERR_ARG, who + "dimension too large");
+    if (!is_fp8_type(d.a_type) || !is_fp8_type(d.b_type)) return fail(ACCB_ERR_ARG, who + "A and B are ACCB_E4M3 or ACCB_E5M2");
+    if (!is_float_type(d.c_type)) return fail(ACCB_ERR_ARG, who + "C is fp32, fp16 or bf16");
+    for (int i = 0; i < 2; ++i)
+        if (d.a_stride[i] < 1 || d.b_stride[i] < 1 || d.c_stride[i] < 1 || scales->a_stride[i] < 1 || scales->b_stride[i] < 1)
+            return fail(ACCB_ERR_ARG, who + "strides must be positive");
+    if ((scales->a_block != 1 && scales->a_block != ACCB_FP8_BLOCK) || (scales->b_block != 1 && scales->b_block != ACCB_FP8_BLOCK))
+        return fail(ACCB_ERR_ARG, who + "a_block and b_block must be 1 or 128");
+    if (d.epilogue != ACCB_EPI_NONE && d.epilogue != ACCB_EPI_RELU) return fail(ACCB_ERR_ARG, who + "unknown epilogue");
+    if (d.compute != ACCB_COMPUTE_AUTO && d.compute != ACCB_COMPUTE_SIMT && d.compute != ACCB_COMPUTE_TENSOR)
+        return fail(ACCB_ERR_ARG, who + "compute is ACCB_COMPUTE_AUTO, ACCB_COMPUTE_SIMT or ACCB_COMPUTE_TENSOR");
+    if (d.max_ctas < 0) return fail(ACCB_ERR_ARG, who + "max_ctas must be >= 0");
+    if (d.m == 0 || d.n == 0) return ACCB_OK;
+    if (!c || (d.k > 0 && (!a || !b || !a_scales || !b_scales))) return fail(ACCB_ERR_ARG, who + "null array pointer");
+
+    DeviceState* sp = nullptr;
+    int dev = 0;
+    int rc = device_state(&sp, &dev);
+    if (rc != ACCB_OK) return rc;
+    DeviceState& s = *sp;
+    const bool on_device = is_device_pointer(c);
+    const void* others[5] = { d.k ? a : c, d.k ? b : c, d.k ? (const void*)a_scales : c, d.k ? (const void*)b_scales : c, bias ? (const void*)bias : c };
+    for (const void* p : others)
+        if (is_device_pointer(p) != on_device) return fail(ACCB_ERR_ARG, who + "mix of host and device pointers");
+
+    GemmFp8Launch g;
+    g.d = d;
+    g.s = *scales;
+    g.a = a; g.b = b; g.c = c; g.a_scales = a_scales; g.b_scales = b_scales; g.bias = bias;
+    g.stream = t_stream;
+    g.status = s.status;
+    g.launch_id = next_launch_id();
+    g.device = dev;
+    g.num_sms = s.num_sms;
+    const char* err = "";
+    if (on_device) {
+        const int n = dispatch_gemm_fp8(g, &err);
+        return n < 0 ? fail(n, who + err) : ACCB_OK;
+    }
+    std::lock_guard<std::mutex> lock(s.mu);
+    const int64_t kb = (d.k + ACCB_FP8_BLOCK - 1) / ACCB_FP8_BLOCK;
+    const size_t bytes[kSlots] = {
+        (size_t)span_elems(d.m, d.k, d.a_stride), (size_t)span_elems(d.k, d.n, d.b_stride),
+        (size_t)span_elems(d.m, d.n, d.c_stride) * type_bytes(d.c_type), bias ? (size_t)d.n * 4 : 0,
+        (size_t)span_elems((d.m + scales->a_block - 1) / scales->a_block, kb, scales->a_stride) * 4,
+        (size_t)span_elems(kb, (d.n + scales->b_block - 1) / scales->b_block, scales->b_stride) * 4 };
+    const void* host[kSlots] = { a, b, c, bias, a_scales, b_scales };
+    const bool c_dense = bytes[2] == (size_t)d.m * (size_t)d.n * type_bytes(d.c_type);
+    for (int i = 0; i < kSlots; ++i) {
+        if (!bytes[i]) continue;
+        if ((rc = ensure(&s.slot[i], &s.slot_bytes[i], bytes[i])) != ACCB_OK) return rc;
+    }
+    for (int i = 0; i < kSlots; ++i) {
+        if (!bytes[i] || (i == 2 && d.beta == 0.0f && c_dense)) continue;
+        const cudaError_t e = cudaMemcpyAsync(s.slot[i], host[i], bytes[i], cudaMemcpyHostToDevice, g.stream);
+        if (e != cudaSuccess) return fail_cuda("host to device copy", e);
+    }
+    g.a = s.slot[0]; g.b = s.slot[1]; g.c = s.slot[2]; g.bias = bias ? (const float*)s.slot[3] : nullptr;
+    g.a_scales = (const float*)s.slot[4]; g.b_scales = (const float*)s.slot[5];
+    const int n = dispatch_gemm_fp8(g, &err);
+    if (n < 0) return fail(n, who + err);
+    const cudaError_t e = cudaMemcpyAsync(c, s.slot[2], bytes[2], cudaMemcpyDeviceToHost, g.stream);
+    if (e != cudaSuccess) return fail_cuda("device to host copy", e);
+    return collect_status(s, g.stream, COLLECT_GEMM, g.launch_id);
+}
+
 int64_t accb_range_count_f32(float start, float limit, float delta)
 {
     return range_count_f32(start, limit, delta);
@@ -897,9 +1150,9 @@ int accb_debug_decode_status(const int32_t* words, int32_t what, int32_t launch_
     if (!words) return ACCB_ERR_ARG;
     int w[kStatusWords];
     for (int i = 0; i < kStatusWords; ++i) w[i] = words[i];
-    bool cg = false, ca = false;
+    bool cg = false, ca = false, ce = false;
     std::string msg;
-    const int rc = decode_status(w, what, launch_id, &cg, &ca, &msg);
+    const int rc = decode_status(w, what, launch_id, &cg, &ca, &ce, &msg);
     if (message && capacity > 0) { strncpy(message, msg.c_str(), (size_t)capacity - 1); message[capacity - 1] = 0; }
     return rc;
 }
@@ -934,7 +1187,7 @@ int accb_release_workspace(void)
     std::lock_guard<std::mutex> lock(s.mu);
     cudaError_t e = cudaDeviceSynchronize();
     if (e != cudaSuccess) return fail_cuda("cudaDeviceSynchronize", e);
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kSlots; ++i) {
         if (s.slot[i]) cudaFree(s.slot[i]);
         s.slot[i] = nullptr;
         s.slot_bytes[i] = 0;
@@ -942,6 +1195,7 @@ int accb_release_workspace(void)
     if (s.scratch) cudaFree(s.scratch);
     s.scratch = nullptr;
     s.scratch_bytes = 0;
+    if (s.pool) cudaMemPoolTrimTo(s.pool, 0);
     return ACCB_OK;
 }
 

@@ -20,8 +20,11 @@ namespace accb {
 //   [3] tcgen05 GEMM: launch id of the launch that recorded [1] and [2]; 0 = no failure recorded
 //   [4] tcgen05 GEMM: number of waits that ran out since the last collection (all launches)
 //   [5] gather: launch id of the last launch that met a bad index
+//   [6] embedding: number of token ids found outside [0, vocab) since the last collection
+//   [7] embedding: launch id of the last launch that met one
 constexpr int kStatusWords = 8;
-enum { ST_GATHER_COUNT = 0, ST_GEMM_SITE = 1, ST_GEMM_STEP = 2, ST_GEMM_ID = 3, ST_GEMM_COUNT = 4, ST_GATHER_ID = 5 };
+enum { ST_GATHER_COUNT = 0, ST_GEMM_SITE = 1, ST_GEMM_STEP = 2, ST_GEMM_ID = 3, ST_GEMM_COUNT = 4, ST_GATHER_ID = 5,
+       ST_EMBED_COUNT = 6, ST_EMBED_ID = 7 };
 // The status buffer is followed by kPaceSlots counters: one per in-flight tensor-core GEMM launch,
 // used to keep its persistent CTAs roughly in step (see gemm_umma.cu).
 constexpr int kPaceSlots = 64;
@@ -146,6 +149,45 @@ int launch_reduce_mean(const float* data, int64_t d0, int64_t d1, int64_t d2, fl
 // gather.cu
 int launch_gather(const void* data, int64_t d0, int64_t d1, const int64_t* indices, int64_t i0, int64_t i1,
                   void* output, int axis, int elem_bytes, int* status, int launch_id, cudaStream_t stream, const char** err);
+
+// embedding.cu: token table lookup and its gradient (device pointers, arguments checked by the caller)
+struct EmbeddingLaunch {
+    accb_embedding_desc d;
+    const void* ids;
+    cudaStream_t stream;
+    int* status;
+    int launch_id;
+    int num_sms;
+    int device;
+};
+int launch_embedding(const EmbeddingLaunch& l, const void* table, void* rows, const char** err);
+int launch_embedding_grad(const EmbeddingLaunch& l, const void* rows, void* table, const char** err);
+
+// quantize_fp8.cu
+int launch_quantize_fp8(const accb_quantize_fp8_desc& d, const void* x, void* q, float* scales, cudaStream_t stream, const char** err);
+
+// gemm_fp8.cu / gemm_fp8_simt.cu
+struct GemmFp8Launch {
+    accb_gemm_desc d;
+    accb_fp8_scales s;
+    const void* a;
+    const void* b;
+    void* c;
+    const float* a_scales;
+    const float* b_scales;
+    const float* bias;
+    cudaStream_t stream;
+    int* status;
+    int launch_id;
+    int device;
+    int num_sms;
+};
+int launch_gemm_fp8_simt(const GemmFp8Launch& g, const char** err);
+
+// Stream-ordered temporaries of the library's own pool on `device` (kept across synchronisations, trimmed by
+// accb_release_workspace): null when there is no memory.
+void* temp_alloc(int device, size_t bytes, cudaStream_t stream);
+void temp_free(void* p, cudaStream_t stream);
 
 // range.cu: output[i] = start + i rounded additions of delta (bit-identical to the serial recurrence); writes the
 // value after n additions to *final_value (host memory).  range_count_f32 is host-only.

@@ -20,7 +20,8 @@ import numpy as np
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libaccera_b200.so")
 
-F32, F16, BF16, S8, S32, U8, S16 = 0, 1, 2, 3, 4, 5, 6
+F32, F16, BF16, S8, S32, U8, S16, E4M3, E5M2 = 0, 1, 2, 3, 4, 5, 6, 7, 8
+FP8_BLOCK = 128          # elements of K that share one scale in quantize_fp8 and gemm_fp8
 COMPUTE_AUTO, COMPUTE_SIMT, COMPUTE_TENSOR, COMPUTE_TENSOR_2SM, COMPUTE_TENSOR_PREFERRED = 0, 1, 2, 3, 4
 EPI_NONE, EPI_RELU = 0, 1
 ERR_ARG, ERR_CUDA, ERR_INDEX, ERR_TIMEOUT, ERR_LIMIT = -1, -2, -3, -4, -5
@@ -32,7 +33,7 @@ _COMPUTE = {"auto": COMPUTE_AUTO, "simt": COMPUTE_SIMT, "tensor": COMPUTE_TENSOR
 
 EXPORTED_SYMBOLS = (
     "accb_gemm", "accb_gemm_batched", "accb_gemm_tile_plan", "accb_gemm_launch_geometry", "accb_gemm_replicated", "accb_reduce_mean_rank3", "accb_reduce_mean_rank3_noalloc", "accb_reduce_mean_rank3_dims", "accb_gather_rank2",
-    "accb_gather_rank2_dims", "accb_range_count_f32", "accb_range_f32", "accb_range_plan_f32", "accb_set_device", "accb_get_device", "accb_current_device", "accb_set_stream", "accb_synchronize", "accb_last_error",
+    "accb_gather_rank2_dims", "accb_embedding", "accb_embedding_grad", "accb_quantize_fp8", "accb_gemm_fp8", "accb_range_count_f32", "accb_range_f32", "accb_range_plan_f32", "accb_set_device", "accb_get_device", "accb_current_device", "accb_set_stream", "accb_synchronize", "accb_last_error",
     "accb_launch_count", "accb_release_workspace", "accb_device_count", "accb_version", "accb_set_option", "accb_debug_decode_status",
 )
 
@@ -54,6 +55,27 @@ class GemmDesc(ctypes.Structure):
         ("alpha", ctypes.c_float), ("beta", ctypes.c_float),
         ("epilogue", ctypes.c_int32), ("max_ctas", ctypes.c_int32),
     ]
+
+
+class EmbeddingDesc(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int64), ("vocab", ctypes.c_int64), ("dim", ctypes.c_int64),
+        ("table_type", ctypes.c_int32), ("rows_type", ctypes.c_int32), ("id_bytes", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64), ("rows_stride", ctypes.c_int64), ("padding_id", ctypes.c_int64),
+        ("scale", ctypes.c_float), ("beta", ctypes.c_float),
+    ]
+
+
+class QuantizeFp8Desc(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("cols", ctypes.c_int64),
+        ("x_type", ctypes.c_int32), ("q_type", ctypes.c_int32), ("block_rows", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("x_stride", ctypes.c_int64 * 2), ("q_stride", ctypes.c_int64), ("scale_stride", ctypes.c_int64 * 2),
+    ]
+
+
+class Fp8Scales(ctypes.Structure):
+    _fields_ = [("a_block", ctypes.c_int32), ("b_block", ctypes.c_int32), ("a_stride", ctypes.c_int64 * 2), ("b_stride", ctypes.c_int64 * 2)]
 
 
 _lib: Optional[ctypes.CDLL] = None
@@ -93,6 +115,14 @@ def lib() -> ctypes.CDLL:
     L.accb_gather_rank2.restype = ctypes.c_int
     L.accb_gather_rank2_dims.argtypes = [i64, i64, i64, i64, i32, ctypes.POINTER(i64)]
     L.accb_gather_rank2_dims.restype = ctypes.c_int
+    L.accb_embedding.argtypes = [ctypes.POINTER(EmbeddingDesc), vp, vp, vp]
+    L.accb_embedding.restype = ctypes.c_int
+    L.accb_embedding_grad.argtypes = [ctypes.POINTER(EmbeddingDesc), vp, vp, vp]
+    L.accb_embedding_grad.restype = ctypes.c_int
+    L.accb_quantize_fp8.argtypes = [ctypes.POINTER(QuantizeFp8Desc), vp, vp, vp]
+    L.accb_quantize_fp8.restype = ctypes.c_int
+    L.accb_gemm_fp8.argtypes = [ctypes.POINTER(GemmDesc), ctypes.POINTER(Fp8Scales), vp, vp, vp, vp, vp, vp]
+    L.accb_gemm_fp8.restype = ctypes.c_int
     L.accb_range_count_f32.argtypes = [ctypes.c_float, ctypes.c_float, ctypes.c_float]
     L.accb_range_count_f32.restype = ctypes.c_int64
     L.accb_range_plan_f32.argtypes = [ctypes.c_float, ctypes.c_float, i64, vp, vp, vp, i64, vp]
@@ -516,6 +546,213 @@ def gather_rank2(data, indices, output, axis: int = 0) -> None:
         raise TypeError("output element size differs from data element size")
     _sync_torch_stream(data, indices, output)
     _check(lib().accb_gather_rank2(pd, shd[0], shd[1], pi, shi[0], shi[1], po, int(axis), int(esize)))
+
+
+# ---------------------------------------------------------------------------
+# token table and 8-bit floating point
+# ---------------------------------------------------------------------------
+
+_FLOAT_KINDS = {"float32": F32, "float16": F16, "bfloat16": BF16}
+_FP8_KINDS = {"float8_e4m3fn": E4M3, "float8_e4m3": E4M3, "float8_e5m2": E5M2}
+_TORCH_CODES: dict = {}
+
+
+def _torch_code(dtype):
+    if not _TORCH_CODES:
+        import torch
+        _TORCH_CODES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3,
+                             torch.float8_e5m2: E5M2, torch.int32: S32, torch.int64: None})
+    try:
+        return _TORCH_CODES[dtype]
+    except KeyError:
+        raise TypeError(f"unsupported tensor dtype {dtype}") from None
+
+
+def _operand(name: str, x, accepted, kind: Optional[str] = None):
+    """-> (pointer, element type code, shape, element strides, device index or -1 for host memory) of an array whose type
+    is one of `accepted` (type codes).  bf16 and 8-bit floating point numpy arrays are bit patterns (uint16, uint8) that `kind` names."""
+    if _is_torch(x):
+        code = _torch_code(x.dtype)
+        if kind is not None and code != _FLOAT_KINDS.get(kind, _FP8_KINDS.get(kind, -1)):
+            raise TypeError(f"{name}: a tensor of {x.dtype} is not {kind}")
+        desc = x.data_ptr(), code, x.shape, x.stride(), (x.device.index if x.is_cuda else -1)
+    elif isinstance(x, np.ndarray):
+        if kind == "bfloat16" and x.dtype == np.uint16:
+            code = BF16
+        elif kind in _FP8_KINDS and x.dtype == np.uint8:
+            code = _FP8_KINDS[kind]
+        elif kind is None or _FLOAT_KINDS.get(kind) == _NP_TYPE.get(str(x.dtype), -1):
+            code = None if x.dtype == np.int64 else _NP_TYPE.get(str(x.dtype), -1)
+        else:
+            raise TypeError(f"{name}: an array of {x.dtype} is not {kind}")
+        if any(st % x.itemsize for st in x.strides):
+            raise ValueError(f"{name}: strides must be whole elements")
+        desc = x.ctypes.data, code, x.shape, tuple(st // x.itemsize for st in x.strides), -1
+    else:
+        raise TypeError(f"{name}: expected a numpy array or a torch tensor")
+    if code not in accepted:
+        raise TypeError(f"{name}: unsupported element type {x.dtype}")
+    return desc
+
+
+_FLOATS = (F32, F16, BF16)
+_FP8 = (E4M3, E5M2)
+
+
+def _select_for(arrays, devices) -> None:
+    """Checks that all arrays are in one place and selects its device and torch's current stream (host: the default stream)."""
+    if any(d != devices[0] for d in devices):
+        raise ValueError("arrays must all be on one device, or all in host memory")
+    _sync_torch_stream(arrays[0])
+
+
+def _positive(strides, shape):
+    """Strides of a descriptor: those of dimensions of length 0 or 1 say nothing and become at least 1."""
+    for st, n in zip(strides, shape):
+        if st < 1 and n > 1:
+            raise ValueError("strides must be positive (no broadcast or reversed dimension)")
+    return [st if st > 0 else 1 for st in strides]
+
+
+def _row_stride(name, shape, strides) -> int:
+    if shape[1] > 1 and strides[1] != 1:
+        raise ValueError(f"{name}: rows must be contiguous")
+    if shape[0] > 1 and strides[0] < shape[1]:
+        raise ValueError(f"{name}: rows must not overlap")
+    return strides[0] if shape[0] > 1 else max(1, shape[1])
+
+
+def _embedding_args(table, ids, rows, scale, beta, padding_id, table_kind, rows_kind):
+    pt, tt, sht, stt, dt = _operand("table", table, _FLOATS, table_kind)
+    pi, ti, shi, sti, di = _operand("ids", ids, (None, S32))
+    pr, tr, shr, str_, dr = _operand("rows", rows, _FLOATS, rows_kind)
+    if len(sht) != 2:
+        raise ValueError("table must be rank 2")
+    if tuple(shr) != tuple(shi) + (sht[1],):
+        raise ValueError(f"shape mismatch: table{tuple(sht)} ids{tuple(shi)} rows{tuple(shr)}")
+    tokens = 1
+    expected = 1
+    for n, st in zip(reversed(shi), reversed(sti)):
+        if n > 1 and st != expected:
+            raise ValueError("ids must be contiguous")
+        expected *= n
+        tokens *= n
+    if len(shr) == 2:
+        shape2, strides2 = shr, str_
+    else:
+        # leading dimensions must fold into one: rows a fixed distance apart
+        lead = [(n, st) for n, st in zip(shr[:-1], str_[:-1]) if n > 1]
+        for (_, outer), (n, inner) in zip(lead, lead[1:]):
+            if outer != n * inner:
+                raise ValueError("rows: the leading dimensions must be evenly spaced rows")
+        shape2, strides2 = (tokens, shr[-1]), (lead[-1][1] if lead else sht[1], str_[-1])
+    d = EmbeddingDesc(tokens, sht[0], sht[1], tt, tr, 8 if ti is None else 4, 0,
+                      _row_stride("table", sht, stt) if tokens else max(1, sht[1]), _row_stride("rows", shape2, strides2) if tokens else max(1, sht[1]),
+                      -1 if padding_id is None else int(padding_id), scale, beta)
+    _select_for((rows, table, ids), (dr, dt, di))
+    return d, pt, pi, pr
+
+
+def embedding(table, ids, out, *, scale: float = 1.0, table_kind: Optional[str] = None, out_kind: Optional[str] = None) -> None:
+    """out[..., :] <- scale * table[ids[...], :].
+
+    table [vocab, dim] and out [*ids.shape, dim] in fp32, fp16 or bf16 (each its own; arithmetic in fp32, one rounding), rows
+    contiguous, any distance apart; ids int32 or int64, contiguous.  An id outside the table gives a row of zeros and
+    AccbError(ERR_INDEX), for CUDA tensors from the next `synchronize()`.  `table_kind` / `out_kind` = "bfloat16" marks
+    uint16 numpy arrays as bf16 bit patterns.
+    """
+    d, pt, pi, po = _embedding_args(table, ids, out, scale, 0.0, None, table_kind, out_kind)
+    _check(lib().accb_embedding(ctypes.byref(d), pt, pi, po))
+
+
+def embedding_grad(grad_out, ids, grad_table, *, scale: float = 1.0, beta: float = 0.0, padding_id: Optional[int] = None,
+                   out_kind: Optional[str] = None, table_kind: Optional[str] = None) -> None:
+    """grad_table[v, :] <- beta * grad_table[v, :] + scale * sum of grad_out[t, :] over the tokens t with ids[t] == v.
+
+    The gradient of `embedding`; shapes and types as there.  Sums are fp32, in an order that the token positions fix, so
+    equal inputs give equal bits.  beta = 0 overwrites the whole table (words without a token become zero), beta = 1 adds to
+    it - the second use of a table that is also the output layer.  Tokens with id `padding_id` add nothing.
+    """
+    if padding_id is not None and padding_id < 0:
+        raise ValueError("padding_id must not be negative (None: no padding)")
+    d, pt, pi, pr = _embedding_args(grad_table, ids, grad_out, scale, beta, padding_id, table_kind, out_kind)
+    _check(lib().accb_embedding_grad(ctypes.byref(d), pr, pi, pt))
+
+
+def _block_of(what: str, blocks: int, count: int) -> int:
+    if blocks == count:
+        return 1
+    if blocks == -(-count // FP8_BLOCK):
+        return FP8_BLOCK
+    raise ValueError(f"{what}: {blocks} scales for {count}: expected one each or one for every {FP8_BLOCK}")
+
+
+def quantize_fp8(x, q, scales, *, kind: Optional[str] = None, q_kind: Optional[str] = None) -> None:
+    """q, scales <- x in 8-bit floating point with one fp32 scale for each group; x is about q * scale.
+
+    x [M, K] in fp32, fp16 or bf16, any positive strides; q [M, K] torch.float8_e4m3fn or float8_e5m2 (numpy: uint8 with
+    q_kind = "float8_e4m3" or "float8_e5m2") with contiguous rows; scales fp32 [M, ceil(K / 128)] (a group is 128 neighbours of a row) or
+    [ceil(M / 128), ceil(K / 128)] (a group is a square tile), any positive strides.  Scales are powers of two, so
+    each value is rounded once; infinities and NaN become NaN and leave the scale alone.  `quantize_fp8(x.t(), q, scales)` gives the
+    transposed result with groups down the columns of x: the form a weight-gradient product needs.
+    """
+    px, tx, shx, stx, dx = _operand("x", x, _FLOATS, kind)
+    pq, tq, shq, stq, dq = _operand("q", q, _FP8, q_kind)
+    ps, _, shs, sts, ds = _operand("scales", scales, (F32,))
+    if len(shx) != 2 or tuple(shq) != tuple(shx) or len(shs) != 2:
+        raise ValueError(f"shape mismatch: x{tuple(shx)} q{tuple(shq)} scales{tuple(shs)}")
+    if shs[1] != -(-shx[1] // FP8_BLOCK):
+        raise ValueError(f"scales{tuple(shs)} must have ceil(K / {FP8_BLOCK}) columns for x{tuple(shx)}")
+    d = QuantizeFp8Desc(shx[0], shx[1], tx, tq, _block_of("scales", shs[0], shx[0]), 0)
+    d.x_stride[:] = _positive(stx, shx)
+    d.q_stride = _row_stride("q", shq, stq)
+    d.scale_stride[:] = _positive(sts, shs)
+    _select_for((x, q, scales), (dx, dq, ds))
+    _check(lib().accb_quantize_fp8(ctypes.byref(d), px, pq, ps))
+
+
+def gemm_fp8(A, B, C, a_scales, b_scales, *, bias=None, alpha: float = 1.0, beta: float = 1.0, relu: bool = False,
+             compute: str = "auto", a_kind: Optional[str] = None, b_kind: Optional[str] = None, out_kind: Optional[str] = None,
+             max_ctas: int = 0) -> None:
+    """C <- epi(alpha * sum_b a_scales[:, b] * b_scales[b, :] * (A[:, b] @ B[b, :]) + beta * C + bias), in place in C,
+    where b runs over the blocks of 128 along K.
+
+    A [M, K] and B [K, N] in torch.float8_e4m3fn or float8_e5m2 (numpy: uint8 with a_kind / b_kind = "float8_e4m3" or
+    "float8_e5m2"), C [M, N] in fp32, fp16 or bf16; strides are taken from the arrays, so a weight matrix stored [N, K] is passed as its
+    transposed view.  a_scales fp32 [M, ceil(K / 128)] or [ceil(M / 128), ceil(K / 128)], b_scales fp32 [ceil(K / 128), N] or
+    [ceil(K / 128), ceil(N / 128)], as `quantize_fp8` writes them (B's transposed like B itself).  Sums are fp32.
+    """
+    pa, ta, sha, sta, da = _operand("A", A, _FP8, a_kind)
+    pb, tb, shb, stb, db = _operand("B", B, _FP8, b_kind)
+    pc, tc, shc, stc, dc = _operand("C", C, _FLOATS, out_kind)
+    psa, _, shsa, stsa, dsa = _operand("a_scales", a_scales, (F32,))
+    psb, _, shsb, stsb, dsb = _operand("b_scales", b_scales, (F32,))
+    if not len(sha) == len(shb) == len(shc) == len(shsa) == len(shsb) == 2:
+        raise ValueError("gemm_fp8 operands and scales must be rank 2")
+    m, k = sha
+    n = shb[1]
+    if shb[0] != k or shc[0] != m or shc[1] != n:
+        raise ValueError(f"shape mismatch: A{tuple(sha)} B{tuple(shb)} C{tuple(shc)}")
+    blocks = -(-k // FP8_BLOCK)
+    if shsa[1] != blocks or shsb[0] != blocks:
+        raise ValueError(f"scales of A{tuple(shsa)} and B{tuple(shsb)} must cover {blocks} blocks of K")
+    devices = [dc, da, db, dsa, dsb]
+    pbias = None
+    if bias is not None:
+        pbias, _, shbias, stbias, dbias = _operand("bias", bias, (F32,))
+        if tuple(shbias) != (n,) or (n > 1 and stbias[0] != 1):
+            raise ValueError("bias must be contiguous fp32 of length N")
+        devices.append(dbias)
+    d = GemmDesc(m, n, k, ta, tb, tc, _COMPUTE[compute])
+    d.a_stride[:] = _positive(sta, sha)
+    d.b_stride[:] = _positive(stb, shb)
+    d.c_stride[:] = _positive(stc, shc)
+    d.alpha, d.beta, d.epilogue, d.max_ctas = alpha, beta, EPI_RELU if relu else EPI_NONE, max_ctas
+    s = Fp8Scales(_block_of("a_scales", shsa[0], m), _block_of("b_scales", shsb[1], n))
+    s.a_stride[:] = _positive(stsa, shsa)
+    s.b_stride[:] = _positive(stsb, shsb)
+    _select_for((C,), devices)
+    _check(lib().accb_gemm_fp8(ctypes.byref(d), ctypes.byref(s), pa, pb, pc, psa, psb, pbias))
 
 
 def range_count(start, limit, delta) -> int:

@@ -37,8 +37,13 @@ enum {
     ACCB_S8 = 3,
     ACCB_S32 = 4,
     ACCB_U8 = 5,
-    ACCB_S16 = 6   /* int16 inputs accumulate exactly into int32 on the CUDA cores (no tensor-core path) */
+    ACCB_S16 = 6,  /* int16 inputs accumulate exactly into int32 on the CUDA cores (no tensor-core path) */
+    ACCB_E4M3 = 7, /* 8-bit floating point, 4 exponent and 3 mantissa bits, no infinity (accb_quantize_fp8, accb_gemm_fp8) */
+    ACCB_E5M2 = 8  /* 8-bit floating point, 5 exponent and 2 mantissa bits (accb_quantize_fp8, accb_gemm_fp8) */
 };
+
+/* elements of K that share one scale in the 8-bit floating point entry points */
+#define ACCB_FP8_BLOCK 128
 
 /* how a GEMM is computed */
 enum {
@@ -62,7 +67,7 @@ enum {
     ACCB_OK = 0,
     ACCB_ERR_ARG = -1,       /* bad descriptor, null pointer, unsupported combination */
     ACCB_ERR_CUDA = -2,      /* a CUDA call failed (no device, out of memory, launch error) */
-    ACCB_ERR_INDEX = -3,     /* gather met an index outside [0, dim): that row was zero-filled */
+    ACCB_ERR_INDEX = -3,     /* gather / embedding met an index outside [0, dim): that row was zero-filled (left out of a gradient) */
     ACCB_ERR_TIMEOUT = -4,   /* a bounded device-side wait ran out; results are invalid */
     ACCB_ERR_LIMIT = -5      /* a fixed-capacity resource is too small for the request */
 };
@@ -218,6 +223,97 @@ int accb_gather_rank2(const void* data, int64_t d0, int64_t d1, const int64_t* i
 
 /* host-only helper: output dims of the gather above */
 int accb_gather_rank2_dims(int64_t d0, int64_t d1, int64_t i0, int64_t i1, int32_t axis, int64_t* out_dims);
+
+/*
+ * Token table: lookup with a scale, and its gradient.  (No counterpart in the reference, whose gather copies elements.)
+ *
+ *   accb_embedding        rows[t, :]  = scale * table[ids[t], :]
+ *   accb_embedding_grad   table[v, :] = beta * table[v, :] + scale * sum of rows[t, :] over the tokens t with ids[t] == v
+ *
+ * `table` is vocab x dim, `rows` tokens x dim; both have unit stride along dim and `*_stride` elements between rows
+ * (at least dim).  Types: ACCB_F32, ACCB_F16 or ACCB_BF16, each side its own; arithmetic is fp32 and each result is
+ * rounded once.  ids is a dense array of `tokens` integers of id_bytes (4 or 8) bytes.
+ *
+ * The gradient adds the rows of one word in an order that depends on the token positions alone (sorted tokens, no
+ * floating-point atomics): the same inputs give the same bits on every run.  With beta = 0 the old table is not read and
+ * words without a token become zero; with beta = 1 such words keep their bytes.  Tokens whose id equals padding_id
+ * (any negative value: none) add nothing, as for any other word their row still gets beta * table.
+ *
+ * An id outside [0, vocab) is not dereferenced: its row is zero-filled (lookup) or left out (gradient) and
+ * ACCB_ERR_INDEX is reported, from this call for host pointers and from the next accb_synchronize() for device
+ * pointers.  Neither array may overlap the other.  A device-pointer accb_embedding_grad takes its workspace (16 bytes a
+ * token and some partial sums) from a stream-ordered pool of the library, so calls on several streams do not share it.
+ * tokens and vocab are below 2^31 - 1, dim is at most 2^20.
+ */
+typedef struct accb_embedding_desc {
+    int64_t tokens, vocab, dim;
+    int32_t table_type, rows_type;
+    int32_t id_bytes;
+    int32_t reserved;                /* 0 */
+    int64_t table_stride, rows_stride;
+    int64_t padding_id;              /* gradient only */
+    float scale;
+    float beta;                      /* gradient only */
+} accb_embedding_desc;
+
+int accb_embedding(const accb_embedding_desc* desc, const void* table, const void* ids, void* rows);
+int accb_embedding_grad(const accb_embedding_desc* desc, const void* rows, const void* ids, void* table);
+
+/*
+ * Quantisation to 8-bit floating point with one fp32 scale for each group of block_rows x 128 values
+ * (block_rows = 1: 128 neighbours of a row; 128: a square tile).  (No counterpart in the reference.)
+ *
+ *   s = 2^e with the smallest e for which max|group| <= top * 2^e   (top = 448 for ACCB_E4M3, 57344 for ACCB_E5M2)
+ *   q = x / s rounded to the nearest 8-bit value, ties to even
+ *
+ * A power of two makes the division exact, so q is rounded once, and q * s never exceeds the largest value.  e is kept
+ * in [-126, 127]; a group of zeros gets s = 1.  Infinities and NaN do not take part in the maximum and become NaN.
+ *
+ * x is rows x cols (ACCB_F32, ACCB_F16, ACCB_BF16) with any positive strides; a transposed view (strides {1, ld}) gives
+ * the transposed result with its groups along the other direction, at the same speed.  q is row-major with q_stride elements
+ * between rows; scales is ceil(rows / block_rows) x ceil(cols / 128) with any positive strides.  The last group of a
+ * row or column may be partial.  Host or device pointers as for accb_gemm; no workspace.
+ */
+typedef struct accb_quantize_fp8_desc {
+    int64_t rows, cols;
+    int32_t x_type, q_type;
+    int32_t block_rows;              /* 1 or 128 */
+    int32_t reserved;                /* 0 */
+    int64_t x_stride[2];
+    int64_t q_stride;
+    int64_t scale_stride[2];
+} accb_quantize_fp8_desc;
+
+int accb_quantize_fp8(const accb_quantize_fp8_desc* desc, const void* x, void* q, float* scales);
+
+/*
+ * GEMM of 8-bit floating point operands with one fp32 scale for each block of 128 along K.
+ * (No counterpart in the reference; the descriptor and the epilogue are those of accb_gemm.)
+ *
+ *   C <- epi(alpha * sum over blocks b of K:  sa[i, b] * sb[b, j] * (A[i, b] @ B[b, j])  +  beta * C + bias[j])
+ *
+ * a_type and b_type are ACCB_E4M3 or ACCB_E5M2, each its own; c_type is ACCB_F32, ACCB_F16 or ACCB_BF16; desc->compute is
+ * ACCB_COMPUTE_AUTO, ACCB_COMPUTE_SIMT or ACCB_COMPUTE_TENSOR (which fails where ACCB_COMPUTE_AUTO would take the CUDA
+ * cores); max_ctas bounds the persistent grid as for accb_gemm.  Every product of a block and the sum over
+ * blocks is accumulated in fp32.
+ *
+ * a_scales is ceil(M / a_block) x ceil(K / 128), b_scales ceil(K / 128) x ceil(N / b_block), a_block and b_block each
+ * 1 (a scale per row of A / column of B) or 128, any positive strides; any fp32 value may be a scale.  A product whose
+ * block sum is infinite or NaN stays so.  Activations (a_block = 1) times weights (b_block = 128) is the forward product and, with the
+ * weights' other direction contiguous, the gradient of its input; 1 and 1 is the gradient of its weights.
+ *
+ * Layouts: on the tensor cores each operand is contiguous along K or along its other direction; C has any strides.
+ * Operands whose rows are not 16-byte aligned are copied into aligned rows first, and few-tile problems keep partial
+ * sums, both in stream-ordered temporaries of the library.  Host or device pointers as for accb_gemm.
+ */
+typedef struct accb_fp8_scales {
+    int32_t a_block, b_block;        /* 1 or 128 */
+    int64_t a_stride[2];             /* of a_scales, in elements */
+    int64_t b_stride[2];             /* of b_scales */
+} accb_fp8_scales;
+
+int accb_gemm_fp8(const accb_gemm_desc* desc, const accb_fp8_scales* scales, const void* a, const void* b, void* c,
+                  const float* a_scales, const float* b_scales, const float* bias);
 
 /*
  * Range (the ONNX operator), fp32.  Replaces the two functions of the reference's range-node test
