@@ -20,8 +20,8 @@ LIB_PATH = os.path.join(_PKG, "libaccera_b200.so")
 INCLUDE_DIR = os.path.join(os.path.dirname(_PKG), "include")
 
 SOURCES = ["abi.cu", "gemm_simt.cu", "gemm_umma.cu", "gemm_splitk.cu", "repack.cu", "reduce_mean.cu", "gather.cu", "range.cu",
-           "embedding.cu", "quantize_fp8.cu", "gemm_fp8_simt.cu"]
-HEADERS = ["accb_internal.h", os.path.join(INCLUDE_DIR, "accera_b200.h")]
+           "embedding.cu", "quantize_fp8.cu", "gemm_fp8.cu", "gemm_fp8_simt.cu"]
+HEADERS = ["accb_internal.h", "umma_device.h", os.path.join(INCLUDE_DIR, "accera_b200.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

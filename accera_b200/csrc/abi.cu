@@ -677,6 +677,8 @@ int accb_set_option(const char* name, int64_t value)
     else if (n == "gemm.pdl") o.gemm_pdl = v < 0 ? -1 : (v ? 1 : 0);
     else if (n == "gemm.epi_warps") o.gemm_epi_warps = (v == 4) ? 4 : (v == 8 ? 8 : 0);
     else if (n == "gemm.split_k") o.gemm_split_k = v < 0 ? -1 : (int)v;
+    else if (n == "gemm_fp8.kernel") { if (value < 0 || value > 2) return fail(ACCB_ERR_ARG, "accb_set_option: gemm_fp8.kernel is 0, 1 or 2"); o.gemm_fp8_kernel = v; }
+    else if (n == "gemm_fp8.slices") { if (value != 0 && value != 1 && value != 2 && value != 4 && value != 8) return fail(ACCB_ERR_ARG, "accb_set_option: gemm_fp8.slices is 0, 1, 2, 4 or 8"); o.gemm_fp8_slices = v; }
     else if (n == "stream_kernels.pdl") o.stream_pdl = v < 0 ? -1 : (v ? 1 : 0);
     else if (n == "gemm.c_in") o.gemm_c_in = v < 0 ? -1 : (v ? 1 : 0);
     else if (n == "gemm.verbose") o.gemm_verbose = v ? 1 : 0;
@@ -874,12 +876,12 @@ static int embedding_entry(const char* fn, bool grad, const accb_embedding_desc*
     if (d.tokens < 0 || d.vocab < 0 || d.dim < 0) return fail(ACCB_ERR_ARG, who + "negative dimension");
     const int64_t lim = ((int64_t)1 << 31) - 1;
     if (d.tokens >= lim || d.vocab >= lim || d.dim >= lim) return fail(ACCB_ERR_ARG, who + "dimension too large");
+    if (d.dim > (int64_t)1 << 20) return fail(ACCB_ERR_ARG, who + "dim is at most 2^20");
     if (!is_float_type(d.table_type) || !is_float_type(d.rows_type)) return fail(ACCB_ERR_ARG, who + "table and rows are fp32, fp16 or bf16");
     if (d.id_bytes != 4 && d.id_bytes != 8) return fail(ACCB_ERR_ARG, who + "id_bytes must be 4 or 8");
     if (d.reserved != 0) return fail(ACCB_ERR_ARG, who + "reserved must be 0");
     if ((d.vocab > 1 && d.table_stride < d.dim) || (d.tokens > 1 && d.rows_stride < d.dim))
         return fail(ACCB_ERR_ARG, who + "row strides must be at least dim");
-    if (d.dim > (int64_t)1 << 20) return fail(ACCB_ERR_ARG, who + "dim is at most 2^20");
     if (d.dim == 0 || (grad ? d.vocab : d.tokens) == 0) return ACCB_OK;
     if ((d.vocab > 0 && !table) || (d.tokens > 0 && (!ids || !rows))) return fail(ACCB_ERR_ARG, who + "null array pointer");
 
@@ -999,7 +1001,11 @@ int accb_quantize_fp8(const accb_quantize_fp8_desc* desc, const void* x, void* q
 // Picks the kernel for one 8-bit GEMM on device pointers.  Returns launches made or a negative ACCB_ERR_*.
 static int dispatch_gemm_fp8(const GemmFp8Launch& g, const char** err)
 {
-    if (g.d.compute == ACCB_COMPUTE_TENSOR && g.d.k > 0) { *err = "no tensor-core kernel takes these operands"; return ACCB_ERR_ARG; }
+    if (g.d.compute != ACCB_COMPUTE_SIMT && g.d.k > 0) {
+        const int n = launch_gemm_fp8(g, err);
+        if (n != 0) return n;
+        if (g.d.compute == ACCB_COMPUTE_TENSOR) { *err = "the tensor cores need operands with unit stride along one direction"; return ACCB_ERR_ARG; }
+    }
     return launch_gemm_fp8_simt(g, err);
 }
 

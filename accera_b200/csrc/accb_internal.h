@@ -55,6 +55,8 @@ struct Options {
     int gemm_verbose = 0;            // print the launch plan to stderr
     int host_stage_chunks = 0;       // row chunks of the staged host-pointer GEMM (default 16)
     int reduce_rows_tpr = 0;         // reduce_mean over contiguous segments: threads per output (32, 64, 128 or 256)
+    int gemm_fp8_kernel = 0;         // 8-bit GEMM: 1 = pair kernel, 2 = tile kernel
+    int gemm_fp8_slices = 0;         // tile kernel: K slices (1, 2, 4 or 8)
     int stream_pdl = -1;             // programmatic dependent launch of the reduce / gather / range kernels: 0 off, 1 on
 };
 Options& options();
@@ -183,6 +185,8 @@ struct GemmFp8Launch {
     int num_sms;
 };
 int launch_gemm_fp8_simt(const GemmFp8Launch& g, const char** err);
+// the tensor cores; returns 0 where they do not take the operands (K = 0, an operand without a contiguous direction)
+int launch_gemm_fp8(const GemmFp8Launch& g, const char** err);
 
 // Stream-ordered temporaries of the library's own pool on `device` (kept across synchronisations, trimmed by
 // accb_release_workspace): null when there is no memory.

@@ -1,0 +1,869 @@
+// Tensor-core GEMM of 8-bit floating point operands with one fp32 scale per block of 128 along K, for sm_100a:
+//
+//   C <- epi(alpha * sum over blocks b of (sa[i, b] sb[b, j]) (A[i, b] @ B[b, j])  +  beta * C + bias[j])
+//
+// A block is 128 bytes of K: one swizzle atom, one pipeline stage, four tcgen05.mma (kind::f8f6f4, K = 32 each).  The
+// scales differ from block to block, so the sum over blocks cannot stay in TMEM: every block's product goes to a TMEM
+// buffer of its own, from where the epilogue warps take it with tcgen05.ld and add it, times the product of its two
+// scales, to fp32 sums in registers.  While they do, the tensor core works on the next block in the other buffer.
+//
+// Two kernels:
+//   pair   256 x 256 tiles by CTA pairs (cta_group::2), persistent: every SM multiplies 128 x 256 x 128 a block, in
+//          512 cycles at the nominal 8-bit rate.  Eight epilogue warps hold the sums, 128 fp32 a thread, and spend 64 packed
+//          fused multiply-adds a thread a block on them: two warps a scheduler, about half of its issue slots.
+//   tile   128 x BN tiles by single CTAs for problems with too few large tiles: columns of C (weights) on the 128 TMEM
+//          lanes, rows of C (tokens) on BN = 16 .. 128 accumulator columns, K cut into up to eight slices
+//          that a cluster multiplies side by side and adds, slice by slice, through distributed shared memory.
+// Scales reach shared memory by 4-byte cp.async (any strides), eight blocks ahead, by the warp that also issues the TMA loads.
+//
+// Every wait is bounded as in gemm_umma.cu: one that runs out is recorded, all roles leave, the host reports
+// ACCB_ERR_TIMEOUT.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <atomic>
+#include <cstring>
+#include <type_traits>
+
+#include "accb_internal.h"
+#include "umma_device.h"
+
+namespace accb {
+namespace {
+
+constexpr int kRowsX = 128;                 // TMEM lanes of a CTA
+constexpr int kRing = 8;                    // blocks of scales in shared memory
+
+struct F8Params {
+    int64_t m, n;
+    int64_t cs0, cs1;
+    int64_t sa_row, sa_kb, sb_col, sb_kb;   // strides of the scales
+    const float* sa;
+    const float* sb;
+    const float* bias;
+    float alpha, beta;
+    int relu;
+    int a_shift, b_shift;                   // 0, or 7 where 128 rows of A / columns of B share a scale
+    int a_mn, b_mn;                         // operand contiguous along M / N instead of K
+    int num_kb;
+    uint32_t idesc;
+    int tiles_m, tiles_n, group_m;
+    int slices;                             // tile kernel: CTAs of a cluster that share one tile's K
+    int c_mode;                             // pair kernel: 2 rows of 16-byte vectors, 1 contiguous rows, 0 any strides
+    int* status;
+    int launch_id;
+    unsigned long long wait_ns;
+};
+
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi)
+{
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+    lo = __uint_as_float(a);
+    hi = __uint_as_float(b);
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+// as tmem_wait_ld: the registers pass through the wait so that their uses stay behind it
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+
+// 4 bytes global -> shared, zero where !inside (the source is not read then)
+__device__ __forceinline__ void copy_scale(uint32_t dst, const float* src, bool inside)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(inside ? 4 : 0) : "memory");
+}
+// arrives on the barrier once this thread's copies so far have landed; the barrier counts one arrival a lane
+__device__ __forceinline__ void copies_arrive(uint32_t bar)
+{
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float load_cluster(uint32_t addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// alpha, beta * old, bias and ReLU of one value; a NaN stays NaN
+__device__ __forceinline__ float finish(float acc, float old, float bias, const F8Params& p)
+{
+    float v = acc * p.alpha;
+    if (p.beta != 0.0f) v = fmaf(p.beta, old, v);
+    if (p.bias) v += bias;
+    if (p.relu) v = v < 0.0f ? 0.0f : v;
+    return v;
+}
+
+// ---------------------------------------------------------------------------------
+// pair kernel
+// ---------------------------------------------------------------------------------
+
+struct PairPlan {
+    static constexpr int kThreads = 320;                                // TMA + scales, MMA, eight epilogue warps
+    static constexpr int kBN = 256;
+    static constexpr int kStageBytes = 2 * kRowsX * kSlabBytes;         // 16 KB of A, 16 KB of B (this CTA's half of the columns)
+    static constexpr int kStages = 5;
+    static constexpr int kBoxBytes = 32 * 128;
+    static constexpr int kScaleBytes = (kRowsX + kBN) * 4;
+    static constexpr int kBoxes = kStages * kStageBytes;
+    static constexpr int kScales = kBoxes + 8 * kBoxBytes;
+    static constexpr int kBars = kScales + kRing * kScaleBytes;
+    static constexpr int kTotal = kBars + 512 + 1024;                   // + manual alignment
+    static_assert(kTotal <= 227 * 1024, "shared memory of a CTA");
+};
+
+// One box (32 rows of 128 bytes, this thread's row in `v`) of the tile to C, through shared memory: a row's 16-byte slots
+// are stored at slot ^ (row % 8), so neither the own-row accesses nor the ones along rows collide in banks.
+template <typename TC>
+__device__ __forceinline__ void store_box(float (&v)[128 / sizeof(TC)], uint8_t* box, TC* C, int64_t row0, int64_t col0, int lane, const F8Params& p)
+{
+    constexpr int W = 128 / (int)sizeof(TC), V = 16 / (int)sizeof(TC);
+    if (p.c_mode == 0) {
+        const int64_t row = row0 + lane;
+        if (row < p.m) {
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+                if (col0 + j < p.n) {
+                    TC* d = C + row * p.cs0 + (col0 + j) * p.cs1;
+                    *d = (TC)finish(v[j], p.beta != 0.0f ? (float)*d : 0.0f, p.bias ? __ldg(p.bias + col0 + j) : 0.0f, p);
+                }
+        }
+        return;
+    }
+    const bool vec = p.c_mode == 2;
+    auto slot_of = [&](int r, int s) { return box + r * 128 + ((s ^ (r & 7)) << 4); };
+    if (p.beta != 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + lane / 8, s = lane % 8;
+            const int64_t col = col0 + s * V;
+            if (row0 + r >= p.m || col >= p.n) continue;
+            const TC* src = C + (row0 + r) * p.cs0 + col;
+            if (vec && col + V <= p.n) *reinterpret_cast<uint4*>(slot_of(r, s)) = *reinterpret_cast<const uint4*>(src);
+            else
+                for (int e = 0; e < V; ++e) if (col + e < p.n) reinterpret_cast<TC*>(slot_of(r, s))[e] = src[e];
+        }
+        __syncwarp();
+    }
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        uint8_t* own = slot_of(lane, s);
+        if (p.beta != 0.0f) w = *reinterpret_cast<const uint4*>(own);
+        TC* h = reinterpret_cast<TC*>(&w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const int64_t col = col0 + s * V + e;
+            h[e] = (TC)finish(v[s * V + e], (float)h[e], p.bias && col < p.n ? __ldg(p.bias + col) : 0.0f, p);
+        }
+        *reinterpret_cast<uint4*>(own) = w;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + lane / 8, s = lane % 8;
+        const int64_t col = col0 + s * V;
+        if (row0 + r >= p.m || col >= p.n) continue;
+        TC* dst = C + (row0 + r) * p.cs0 + col;
+        if (vec && col + V <= p.n) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(slot_of(r, s));
+        else
+            for (int e = 0; e < V; ++e) if (col + e < p.n) dst[e] = reinterpret_cast<const TC*>(slot_of(r, s))[e];
+    }
+    __syncwarp();
+}
+
+__device__ __forceinline__ void pair_tile(int t, const F8Params& p, int& tm, int& tn)
+{
+    const int group_size = p.group_m * p.tiles_n;
+    const int group = t / group_size;
+    const int first_m = group * p.group_m;
+    const int rows = min(p.tiles_m - first_m, p.group_m);
+    const int in = t - group * group_size;
+    tm = first_m + in % rows;
+    tn = in / rows;
+}
+
+// COLS: every column of B has a scale of its own (else 128 share one)
+template <typename TC, bool COLS>
+__global__ void __launch_bounds__(PairPlan::kThreads, 1)
+gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, TC* __restrict__ C, const F8Params p)
+{
+    using Plan = PairPlan;
+    constexpr int S = Plan::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+    const uint32_t bars = smem_base + Plan::kBars;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
+    auto tmem_full_bar = [&](int b) { return bars + 8u * (2 * S + b); };
+    auto tmem_empty_bar = [&](int b) { return bars + 8u * (2 * S + 2 + b); };
+    auto scale_full_bar = [&](int r) { return bars + 8u * (2 * S + 4 + r); };
+    auto scale_empty_bar = [&](int r) { return bars + 8u * (2 * S + 4 + kRing + r); };
+    volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(smem_gen + Plan::kBars + 8 * (2 * S + 4 + 2 * kRing));
+    volatile uint32_t* gave_up = tmem_holder + 2;        // one word a CTA of the pair, each CTA with a copy of both
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const WaitCtx wctx{p.status, p.launch_id, p.wait_ns};
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    auto record_give_up = [&]() {
+        gave_up[rank] = 1u;
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to_rank(smem_u32((const void*)(gave_up + rank)), rank ^ 1u)), "r"(1u) : "memory");
+    };
+    if (threadIdx.x == 0) {
+        gave_up[0] = 0u;
+        gave_up[1] = 0u;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_a)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_b)) : "memory");
+        for (int s = 0; s < S; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(tmem_full_bar(b), 1); mbar_init(tmem_empty_bar(b), 16); }   // a commit; the warps of both CTAs
+        for (int r = 0; r < kRing; ++r) { mbar_init(scale_full_bar(r), 32); mbar_init(scale_empty_bar(r), 8); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_holder)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync_all();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *tmem_holder;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const int num_tiles = p.tiles_m * p.tiles_n;
+    const int num_units = (int)gridDim.x / 2, unit = (int)blockIdx.x / 2;
+    const int num_kb = p.num_kb;
+
+    if (warp == 0) {
+        // ---------------- scales by the whole warp, TMA loads by lane 0 ----------------
+        int s = 0, r = 0;
+        uint32_t ph = 0, rph = 0;
+        bool ok = true;
+        for (int t = unit; t < num_tiles && ok; t += num_units) {
+            int tm, tn;
+            pair_tile(t, p, tm, tn);
+            const int row_a = (tm * 2 + (int)rank) * kRowsX, col_b = tn * Plan::kBN, row_b = col_b + (int)rank * 128;
+            const float* src_a[4];
+            bool in_a[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t row = row_a + i * 32 + lane;
+                in_a[i] = row < p.m;
+                src_a[i] = p.sa + (in_a[i] ? (row >> p.a_shift) * p.sa_row : 0);
+            }
+            constexpr int kColLoads = COLS ? 8 : 1;
+            const float* src_b[kColLoads];
+            bool in_b[kColLoads];
+#pragma unroll
+            for (int i = 0; i < kColLoads; ++i) {
+                const int64_t col = COLS ? (int64_t)col_b + i * 32 + lane : (int64_t)col_b + lane * 128;
+                in_b[i] = col < p.n && (COLS || lane < 2);
+                src_b[i] = p.sb + (in_b[i] ? (col >> p.b_shift) * p.sb_col : 0);
+            }
+            for (int kb = 0; kb < num_kb; ++kb) {
+                ok = mbar_wait(scale_empty_bar(r), rph ^ 1u, wctx, SITE_PRODUCER_EMPTY, kb);
+                if (ok) {
+                    const uint32_t sc = smem_base + Plan::kScales + r * Plan::kScaleBytes;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) copy_scale(sc + (i * 32 + lane) * 4, src_a[i] + kb * p.sa_kb, in_a[i]);
+#pragma unroll
+                    for (int i = 0; i < kColLoads; ++i)
+                        if (COLS || lane < 2) copy_scale(sc + (kRowsX + i * 32 + lane) * 4, src_b[i] + kb * p.sb_kb, in_b[i]);
+                    copies_arrive(scale_full_bar(r));
+                    if (++r == kRing) { r = 0; rph ^= 1u; }
+                }
+                if (lane == 0 && ok) {
+                    ok = mbar_wait(empty_bar(s), ph ^ 1u, wctx, SITE_PRODUCER_EMPTY, kb);
+                    if (ok) {
+                        const uint32_t sa = smem_base + s * Plan::kStageBytes, sb = sa + kRowsX * kSlabBytes;
+                        if (leader) mbar_arrive_expect_tx(full_bar(s), 2u * Plan::kStageBytes);
+                        if (p.a_mn) tma_load_2d_pair(sa, &map_a, full_bar(s), row_a, kb * kSlabBytes, 0);
+                        else tma_load_2d_pair(sa, &map_a, full_bar(s), kb * kSlabBytes, row_a, 0);
+                        if (p.b_mn) tma_load_2d_pair(sb, &map_b, full_bar(s), row_b, kb * kSlabBytes, 0);
+                        else tma_load_2d_pair(sb, &map_b, full_bar(s), kb * kSlabBytes, row_b, 0);
+                    }
+                }
+                if (++s == S) { s = 0; ph ^= 1u; }
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+            }
+        }
+        if (!ok && lane == 0) record_give_up();
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (rank 0 of the pair) ----------------
+        if (lane == 0 && leader) {
+            auto issue = [&](auto a_mn_tag, auto b_mn_tag) {
+                constexpr bool A_MN = decltype(a_mn_tag)::value, B_MN = decltype(b_mn_tag)::value;
+                int s = 0, g = 0;
+                uint32_t ph = 0;
+                bool ok = true;
+                for (int t = unit; t < num_tiles && ok; t += num_units) {
+                    for (int kb = 0; kb < num_kb; ++kb, ++g) {
+                        const int buf = g & 1;
+                        if (!mbar_wait(tmem_empty_bar(buf), ((g >> 1) & 1u) ^ 1u, wctx, SITE_MMA_TMEM_EMPTY, kb) ||
+                            !mbar_wait(full_bar(s), ph, wctx, SITE_MMA_FULL, kb)) { ok = false; break; }
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t sa = smem_base + s * Plan::kStageBytes;
+                        issue_stage<KIND_F8F6F4, true, A_MN, B_MN>(tmem_base + (uint32_t)(buf * Plan::kBN), sa, sa + kRowsX * kSlabBytes, p.idesc, true);
+                        umma_commit<true>(empty_bar(s));
+                        umma_commit<true>(tmem_full_bar(buf));
+                        if (++s == S) { s = 0; ph ^= 1u; }
+                    }
+                }
+                if (!ok) record_give_up();
+            };
+            if (!p.a_mn && !p.b_mn) issue(std::false_type{}, std::false_type{});
+            else if (!p.b_mn) issue(std::true_type{}, std::false_type{});
+            else if (!p.a_mn) issue(std::false_type{}, std::true_type{});
+            else issue(std::true_type{}, std::true_type{});
+        }
+    } else {
+        // ---------------- epilogue warps ----------------
+        const int q = warp & 3, ew = warp - 2, half = ew >> 2;      // TMEM lane quarter, half of the tile's columns
+        uint8_t* box = smem_gen + Plan::kBoxes + ew * Plan::kBoxBytes;
+        const float* scales = reinterpret_cast<const float*>(smem_gen + Plan::kScales);
+        const uint32_t taddr0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
+        int g = 0, r = 0;
+        uint32_t rph = 0;
+        bool ok = true;
+        for (int t = unit; t < num_tiles && ok; t += num_units) {
+            int tm, tn;
+            pair_tile(t, p, tm, tn);
+            uint64_t acc[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] = 0ull;
+            for (int kb = 0; kb < num_kb; ++kb, ++g) {
+                const int buf = g & 1;
+                ok = mbar_wait(scale_full_bar(r), rph, wctx, SITE_EPI_TMEM_FULL, kb) &&
+                     mbar_wait(tmem_full_bar(buf), (g >> 1) & 1u, wctx, SITE_EPI_TMEM_FULL, kb);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const float* sc = scales + r * (Plan::kScaleBytes / 4);
+                const float row_scale = sc[q * 32 + lane];
+                const float* col_scale = sc + kRowsX + (COLS ? half * 128 : half);
+                const float f = COLS ? row_scale : row_scale * col_scale[0];
+                const uint64_t f2 = pack2(__float_as_uint(f), __float_as_uint(f));
+                const uint32_t taddr = taddr0 + (uint32_t)(buf * Plan::kBN);
+                uint32_t x[2][16];
+                tmem_ld16(taddr, x[0]);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    tmem_wait_ld16(x[c & 1]);
+                    if (c < 7) tmem_ld16(taddr + (uint32_t)(16 * (c + 1)), x[(c + 1) & 1]);
+                    else {
+                        // this warp has read the buffer: the MMA issuer of the pair may overwrite it
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(tmem_empty_bar(buf) & kPeerMask);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        uint64_t g0 = f2, g1 = f2;
+                        if constexpr (COLS) {
+                            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(col_scale + 16 * c + 2 * j);
+                            g0 = mul2(f2, w.x);
+                            g1 = mul2(f2, w.y);
+                        }
+                        acc[8 * c + j] = fma2(pack2(x[c & 1][2 * j], x[c & 1][2 * j + 1]), g0, acc[8 * c + j]);
+                        acc[8 * c + j + 1] = fma2(pack2(x[c & 1][2 * j + 2], x[c & 1][2 * j + 3]), g1, acc[8 * c + j + 1]);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(scale_empty_bar(r));
+                if (++r == kRing) { r = 0; rph ^= 1u; }
+            }
+            if (!ok) break;
+            const int64_t row0 = (int64_t)(tm * 2 + (int)rank) * kRowsX + q * 32, col0 = (int64_t)tn * Plan::kBN + half * 128;
+            constexpr int W = 128 / (int)sizeof(TC);
+#pragma unroll
+            for (int b = 0; b < 128 / W; ++b) {
+                float v[W];
+#pragma unroll
+                for (int j = 0; j < W; j += 2) unpack2(acc[(b * W + j) / 2], v[j], v[j + 1]);
+                if (row0 < p.m && col0 + b * W < p.n) store_box<TC>(v, box, C, row0, col0 + b * W, lane, p);
+            }
+        }
+        if (!ok && lane == 0) record_give_up();
+    }
+
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync_all();
+    if ((gave_up[0] | gave_up[1]) != 0u) {
+        // give loads that are still in flight time to land before shared memory is released
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);
+        cluster_sync_all();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------------
+// tile kernel
+// ---------------------------------------------------------------------------------
+
+template <int BN> struct TilePlan {
+    static constexpr int kThreads = 192;                                 // TMA + scales, MMA, four epilogue warps
+    static constexpr int kStageBytes = (kRowsX + BN) * kSlabBytes;       // 128 columns of C (weights), BN rows of C (tokens)
+    static constexpr int kStages = BN == 128 ? 3 : BN == 64 ? 4 : BN == 32 ? 5 : 5;
+    static constexpr int kBuffers = BN == 128 ? 2 : BN == 64 ? 4 : 8;    // TMEM accumulators of BN columns
+    static constexpr int kTmemCols = kBuffers * BN;
+    static constexpr int kScaleBytes = (kRowsX + BN) * 4;
+    static constexpr int kScales = kStages * kStageBytes;
+    static constexpr int kBars = kScales + kRing * kScaleBytes;
+    static constexpr int kTotal = kBars + 512 + 1024;
+    static_assert(kTotal <= 113 * 1024, "two CTAs share an SM");
+    static_assert(BN * kRowsX * 4 <= kStages * kStageBytes, "the sums of a slice fit the operand ring");
+};
+
+template <typename TC, int BN>
+__global__ void __launch_bounds__(TilePlan<BN>::kThreads, 2)
+gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_t, TC* __restrict__ C, const F8Params p)
+{
+    using Plan = TilePlan<BN>;
+    constexpr int S = Plan::kStages, NB = Plan::kBuffers;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+    const uint32_t bars = smem_base + Plan::kBars;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
+    auto tmem_full_bar = [&](int b) { return bars + 8u * (2 * S + b); };
+    auto tmem_empty_bar = [&](int b) { return bars + 8u * (2 * S + NB + b); };
+    auto scale_full_bar = [&](int r) { return bars + 8u * (2 * S + 2 * NB + r); };
+    auto scale_empty_bar = [&](int r) { return bars + 8u * (2 * S + 2 * NB + kRing + r); };
+    static_assert(8 * (2 * S + 2 * NB + 2 * kRing) + 16 <= 512, "barriers");
+    volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(smem_gen + Plan::kBars + 8 * (2 * S + 2 * NB + 2 * kRing));
+    volatile uint32_t* gave_up = tmem_holder + 2;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const WaitCtx wctx{p.status, p.launch_id, p.wait_ns};
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x == 0) {
+        gave_up[0] = 0u;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_t)) : "memory");
+        for (int s = 0; s < S; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        for (int b = 0; b < NB; ++b) { mbar_init(tmem_full_bar(b), 1); mbar_init(tmem_empty_bar(b), 4); }
+        for (int r = 0; r < kRing; ++r) { mbar_init(scale_full_bar(r), 32); mbar_init(scale_empty_bar(r), 4); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_holder)), "r"(Plan::kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *tmem_holder;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    // neighbouring tiles share their weights, which are the larger operand
+    const int tile = (int)blockIdx.x / p.slices, slice = (int)blockIdx.x % p.slices;
+    const int row0 = (tile / p.tiles_m) * kRowsX;                        // first column of C (weight)
+    const int col0 = (tile % p.tiles_m) * BN;                            // first row of C (token)
+    const int kb_begin = (int)((int64_t)p.num_kb * slice / p.slices), kb_end = (int)((int64_t)p.num_kb * (slice + 1) / p.slices);
+
+    uint64_t acc[BN / 2];
+#pragma unroll
+    for (int i = 0; i < BN / 2; ++i) acc[i] = 0ull;
+
+    if (warp == 0) {
+        int s = 0, r = 0;
+        uint32_t ph = 0, rph = 0;
+        bool ok = true;
+        const float* src_w[4];
+        bool in_w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t row = (int64_t)row0 + i * 32 + lane;
+            in_w[i] = row < p.n;
+            src_w[i] = p.sb + (in_w[i] ? (row >> p.b_shift) * p.sb_col : 0);
+        }
+        constexpr int kColLoads = (BN + 31) / 32;
+        const float* src_t[kColLoads];
+        bool in_t[kColLoads];
+#pragma unroll
+        for (int i = 0; i < kColLoads; ++i) {
+            const int64_t col = (int64_t)col0 + i * 32 + lane;
+            in_t[i] = col < p.m && i * 32 + lane < BN;
+            src_t[i] = p.sa + (in_t[i] ? (col >> p.a_shift) * p.sa_row : 0);
+        }
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
+            // the operands first: the scales are needed only once a block has been multiplied
+            if (lane == 0) {
+                ok = mbar_wait(empty_bar(s), ph ^ 1u, wctx, SITE_PRODUCER_EMPTY, kb);
+                if (ok) {
+                    const uint32_t sw = smem_base + s * Plan::kStageBytes, st = sw + kRowsX * kSlabBytes;
+                    mbar_arrive_expect_tx(full_bar(s), (uint32_t)Plan::kStageBytes);
+                    if (p.b_mn) tma_load_2d(sw, &map_w, full_bar(s), row0, kb * kSlabBytes, 0);
+                    else tma_load_2d(sw, &map_w, full_bar(s), kb * kSlabBytes, row0, 0);
+                    if (p.a_mn) tma_load_2d(st, &map_t, full_bar(s), col0, kb * kSlabBytes, 0);
+                    else tma_load_2d(st, &map_t, full_bar(s), kb * kSlabBytes, col0, 0);
+                }
+            }
+            if (++s == S) { s = 0; ph ^= 1u; }
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(scale_empty_bar(r), rph ^ 1u, wctx, SITE_PRODUCER_EMPTY, kb));
+            if (!ok) break;
+            const uint32_t sc = smem_base + Plan::kScales + r * Plan::kScaleBytes;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) copy_scale(sc + (i * 32 + lane) * 4, src_w[i] + kb * p.sb_kb, in_w[i]);
+#pragma unroll
+            for (int i = 0; i < kColLoads; ++i)
+                if (i * 32 + lane < BN) copy_scale(sc + (kRowsX + i * 32 + lane) * 4, src_t[i] + kb * p.sa_kb, in_t[i]);
+            copies_arrive(scale_full_bar(r));
+            if (++r == kRing) { r = 0; rph ^= 1u; }
+        }
+        if (!ok && lane == 0) gave_up[0] = 1u;
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp == 1) {
+        if (lane == 0) {
+            auto issue = [&](auto w_mn_tag, auto t_mn_tag) {
+                constexpr bool W_MN = decltype(w_mn_tag)::value, T_MN = decltype(t_mn_tag)::value;
+                int s = 0, b = 0;
+                uint32_t ph = 0, bph = 0;
+                for (int kb = kb_begin; kb < kb_end; ++kb) {
+                    if (!mbar_wait(tmem_empty_bar(b), bph ^ 1u, wctx, SITE_MMA_TMEM_EMPTY, kb) || !mbar_wait(full_bar(s), ph, wctx, SITE_MMA_FULL, kb)) {
+                        gave_up[0] = 1u;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t sw = smem_base + s * Plan::kStageBytes;
+                    issue_stage<KIND_F8F6F4, false, W_MN, T_MN>(tmem_base + (uint32_t)(b * BN), sw, sw + kRowsX * kSlabBytes, p.idesc, true);
+                    umma_commit<false>(empty_bar(s));
+                    umma_commit<false>(tmem_full_bar(b));
+                    if (++s == S) { s = 0; ph ^= 1u; }
+                    if (++b == NB) { b = 0; bph ^= 1u; }
+                }
+            };
+            if (!p.b_mn && !p.a_mn) issue(std::false_type{}, std::false_type{});
+            else if (!p.a_mn) issue(std::true_type{}, std::false_type{});
+            else if constexpr (BN == 128) {                              // an M-contiguous box is 128 wide: the host takes BN = 128 then
+                if (!p.b_mn) issue(std::false_type{}, std::true_type{});
+                else issue(std::true_type{}, std::true_type{});
+            }
+        }
+    } else {
+        const int q = warp & 3;
+        const float* scales = reinterpret_cast<const float*>(smem_gen + Plan::kScales);
+        const uint32_t taddr0 = tmem_base + ((uint32_t)(q * 32) << 16);
+        int b = 0, r = 0;
+        uint32_t bph = 0, rph = 0;
+        bool ok = true;
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
+            ok = mbar_wait(scale_full_bar(r), rph, wctx, SITE_EPI_TMEM_FULL, kb) && mbar_wait(tmem_full_bar(b), bph, wctx, SITE_EPI_TMEM_FULL, kb);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const float* sc = scales + r * (Plan::kScaleBytes / 4);
+            const float f = sc[q * 32 + lane];
+            const uint64_t f2 = pack2(__float_as_uint(f), __float_as_uint(f));
+            const uint32_t taddr = taddr0 + (uint32_t)(b * BN);
+#pragma unroll
+            for (int c = 0; c < BN / 16; ++c) {
+                uint32_t x[16];
+                tmem_ld16(taddr + (uint32_t)(16 * c), x);
+                tmem_wait_ld16(x);
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(sc + kRowsX + 16 * c + 2 * j);
+                    acc[8 * c + j] = fma2(pack2(x[2 * j], x[2 * j + 1]), mul2(f2, w.x), acc[8 * c + j]);
+                    acc[8 * c + j + 1] = fma2(pack2(x[2 * j + 2], x[2 * j + 3]), mul2(f2, w.y), acc[8 * c + j + 1]);
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(tmem_empty_bar(b)); mbar_arrive(scale_empty_bar(r)); }
+            if (++b == NB) { b = 0; bph ^= 1u; }
+            if (++r == kRing) { r = 0; rph ^= 1u; }
+        }
+        if (!ok && lane == 0) gave_up[0] = 1u;
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (gave_up[0] != 0u) {
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Plan::kTmemCols) : "memory");
+    }
+
+    // All loads and MMAs of this CTA are done: the operand ring may hold the slice's sums, [BN][128] fp32.
+    const int64_t n_index = (int64_t)row0 + (warp & 3) * 32 + lane;
+    const int cols = (int)(p.m - col0 < BN ? p.m - col0 : BN);
+    auto put = [&](int c, float v) {
+        if (n_index >= p.n) return;
+        TC* d = C + (col0 + c) * p.cs0 + n_index * p.cs1;
+        *d = (TC)finish(v, p.beta != 0.0f ? (float)*d : 0.0f, p.bias ? __ldg(p.bias + n_index) : 0.0f, p);
+    };
+    if (p.slices == 1) {
+        if (warp >= 2) {
+#pragma unroll
+            for (int c = 0; c < BN; c += 2) {
+                float lo, hi;
+                unpack2(acc[c / 2], lo, hi);
+                if (c < cols) put(c, lo);
+                if (c + 1 < cols) put(c + 1, hi);
+            }
+        }
+        return;
+    }
+    float* sums = reinterpret_cast<float*>(smem_gen);
+    const int at = (warp & 3) * 32 + lane;
+    if (warp >= 2) {
+#pragma unroll
+        for (int c = 0; c < BN; c += 2) {
+            float lo, hi;
+            unpack2(acc[c / 2], lo, hi);
+            sums[c * kRowsX + at] = lo;
+            sums[(c + 1) * kRowsX + at] = hi;
+        }
+    }
+    cluster_sync_all();
+    if (warp >= 2) {
+        // this CTA's share of the columns: every slices-th, the slices' sums added in their order along K
+        for (int c = slice; c < cols; c += p.slices) {
+            float v = 0.0f;
+            for (int z = 0; z < p.slices; ++z) v += load_cluster(map_to_rank(smem_base + (uint32_t)(c * kRowsX + at) * 4, (uint32_t)z));
+            put(c, v);
+        }
+    }
+    cluster_sync_all();                                                  // nobody leaves while its sums are being read
+}
+
+// ---------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------
+
+uint32_t f8_idesc(const accb_gemm_desc& d, bool swapped, int m, int n, bool a_mn, bool b_mn)
+{
+    const int x = swapped ? d.b_type : d.a_type, y = swapped ? d.a_type : d.b_type;
+    const bool x_mn = swapped ? b_mn : a_mn, y_mn = swapped ? a_mn : b_mn;
+    uint32_t i = 1u << 4;                                                // fp32 accumulator
+    i |= (x == ACCB_E5M2 ? 1u : 0u) << 7;
+    i |= (y == ACCB_E5M2 ? 1u : 0u) << 10;
+    i |= (x_mn ? 1u : 0u) << 15;
+    i |= (y_mn ? 1u : 0u) << 16;
+    i |= (uint32_t)(n >> 3) << 17;
+    i |= (uint32_t)(m >> 4) << 24;
+    return i;
+}
+
+constexpr int kMaxDevices = 64;
+
+template <typename TC, bool COLS>
+cudaError_t launch_pair(const GemmFp8Launch& g, const CUtensorMap& ma, const CUtensorMap& mb, const F8Params& p)
+{
+    auto kernel = gemm_fp8_pair_kernel<TC, COLS>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(PairPlan::kThreads);
+    cfg.dynamicSmemBytes = PairPlan::kTotal;
+    cfg.stream = g.stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = options().gemm_pdl == 0 ? 0 : 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    static std::atomic<int> resident[kMaxDevices];
+    int units = g.device < kMaxDevices ? resident[g.device].load(std::memory_order_acquire) : 0;
+    if (units == 0) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PairPlan::kTotal);
+        if (e != cudaSuccess) return e;
+        cfg.gridDim = dim3(2 * (unsigned)(g.num_sms / 2));
+        e = cudaOccupancyMaxActiveClusters(&units, kernel, &cfg);
+        if (e != cudaSuccess) return e;
+        if (units < 1) return cudaErrorLaunchOutOfResources;
+        if (units > g.num_sms / 2) units = g.num_sms / 2;
+        if (g.device < kMaxDevices) resident[g.device].store(units, std::memory_order_release);
+    }
+    if (g.d.max_ctas > 0 && units > (g.d.max_ctas + 1) / 2) units = (g.d.max_ctas + 1) / 2;
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+    if (units > tiles) units = (int)tiles;
+    cfg.gridDim = dim3((unsigned)(2 * units));
+    return cudaLaunchKernelEx(&cfg, kernel, ma, mb, (TC*)g.c, p);
+}
+
+template <typename TC, int BN>
+cudaError_t launch_tile(const GemmFp8Launch& g, const CUtensorMap& mw, const CUtensorMap& mt, const F8Params& p)
+{
+    auto kernel = gemm_fp8_tile_kernel<TC, BN>;
+    static std::atomic<bool> opted[kMaxDevices];
+    if (g.device >= kMaxDevices || !opted[g.device].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TilePlan<BN>::kTotal);
+        if (e != cudaSuccess) return e;
+        if (g.device < kMaxDevices) opted[g.device].store(true, std::memory_order_release);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.tiles_m * p.tiles_n * p.slices));
+    cfg.blockDim = dim3(TilePlan<BN>::kThreads);
+    cfg.dynamicSmemBytes = TilePlan<BN>::kTotal;
+    cfg.stream = g.stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.slices; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = options().gemm_pdl == 0 ? 0 : 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, mw, mt, (TC*)g.c, p);
+}
+
+template <typename TC>
+cudaError_t launch_c(const GemmFp8Launch& g, const CUtensorMap& ma, const CUtensorMap& mb, const F8Params& p, int bn)
+{
+    if (bn == 256) return p.b_shift ? launch_pair<TC, false>(g, ma, mb, p) : launch_pair<TC, true>(g, ma, mb, p);
+    if (bn == 128) return launch_tile<TC, 128>(g, mb, ma, p);
+    if (bn == 64) return launch_tile<TC, 64>(g, mb, ma, p);
+    if (bn == 32) return launch_tile<TC, 32>(g, mb, ma, p);
+    return launch_tile<TC, 16>(g, mb, ma, p);
+}
+
+}  // namespace
+
+// Contiguous direction of an operand [rows, k] with element strides `s_rows`, `s_k`: 0 along K, 1 along its rows, -1 neither.
+// Where both would do (one row, or K = 1) K comes first.
+static int contiguous_direction(int64_t rows, int64_t k, int64_t s_rows, int64_t s_k)
+{
+    if (s_k == 1 || k == 1) return 0;
+    if (s_rows == 1 || rows == 1) return 1;
+    return -1;
+}
+
+int launch_gemm_fp8(const GemmFp8Launch& g0, const char** err)
+{
+    GemmFp8Launch g = g0;
+    const accb_gemm_desc& d = g.d;
+    const int a_dir = contiguous_direction(d.m, d.k, d.a_stride[0], d.a_stride[1]);
+    const int b_dir = contiguous_direction(d.n, d.k, d.b_stride[1], d.b_stride[0]);
+    if (d.k < 1 || a_dir < 0 || b_dir < 0 || !encode_tiled_fn()) return 0;
+
+    // Operands as `lines` runs of `width` bytes, `pitch` bytes apart.  TMA wants 16-byte aligned runs: others are copied.
+    struct Operand { const void* base; int64_t lines, width, pitch; } op[2] = {
+        { g.a, a_dir ? d.k : d.m, a_dir ? d.m : d.k, a_dir ? d.a_stride[1] : d.a_stride[0] },
+        { g.b, b_dir ? d.k : d.n, b_dir ? d.n : d.k, b_dir ? d.b_stride[0] : d.b_stride[1] } };
+    void* tmp[2] = { nullptr, nullptr };
+    auto release = [&]() { for (void* t : tmp) temp_free(t, g.stream); };
+    int launches = 0;
+    for (int i = 0; i < 2; ++i) {
+        Operand& o = op[i];
+        if (o.lines == 1) o.pitch = (o.width + 15) / 16 * 16;            // never followed
+        if (o.pitch % 16 == 0 && (reinterpret_cast<uintptr_t>(o.base) & 15) == 0) continue;
+        const int64_t pitch = (o.width + 15) / 16 * 16;
+        tmp[i] = temp_alloc(g.device, (size_t)(pitch * o.lines), g.stream);
+        if (!tmp[i]) { release(); *err = "no device memory for an aligned copy of an operand"; return ACCB_ERR_CUDA; }
+        const int rc = launch_repack_rows(o.base, o.pitch, o.lines, o.width, 1, tmp[i], pitch, o.lines, g.stream, err);
+        if (rc < 0) { release(); return rc; }
+        launches += rc;
+        o.base = tmp[i];
+        o.pitch = pitch;
+    }
+
+    F8Params p;
+    memset(&p, 0, sizeof p);
+    p.m = d.m; p.n = d.n;
+    p.cs0 = d.c_stride[0]; p.cs1 = d.c_stride[1];
+    p.sa = g.a_scales; p.sb = g.b_scales; p.bias = g.bias;
+    p.sa_row = g.s.a_stride[0]; p.sa_kb = g.s.a_stride[1]; p.sb_kb = g.s.b_stride[0]; p.sb_col = g.s.b_stride[1];
+    p.a_shift = g.s.a_block == 1 ? 0 : 7; p.b_shift = g.s.b_block == 1 ? 0 : 7;
+    p.alpha = d.alpha; p.beta = d.beta; p.relu = d.epilogue == ACCB_EPI_RELU;
+    p.a_mn = a_dir; p.b_mn = b_dir;
+    p.num_kb = (int)((d.k + kSlabBytes - 1) / kSlabBytes);
+    p.status = g.status; p.launch_id = g.launch_id;
+    const Options& o = options();
+    p.wait_ns = o.gemm_wait_limit_us > 0 ? (unsigned long long)o.gemm_wait_limit_us * 1000ull : 1000000000ull;
+
+    const int64_t pair_tiles = ((d.m + 255) / 256) * ((d.n + 255) / 256);
+    bool pair = d.max_ctas > 0 || (d.m > 128 && pair_tiles * 2 > g.num_sms / 2);
+    if (o.gemm_fp8_kernel) pair = o.gemm_fp8_kernel == 1;
+    int bn = 256;
+    if (pair) {
+        p.tiles_m = (int)((d.m + 255) / 256); p.tiles_n = (int)((d.n + 255) / 256);
+        p.group_m = 8;
+        p.idesc = f8_idesc(d, false, 256, 256, a_dir, b_dir);
+        const int es = elem_size(d.c_type);
+        p.c_mode = d.c_stride[1] != 1 ? 0 : (d.c_stride[0] * es % 16 == 0 && (reinterpret_cast<uintptr_t>(g.c) & 15) == 0) ? 2 : 1;
+        if (pair_tiles > 0x3fffffff) { release(); *err = "too many tiles"; return ACCB_ERR_ARG; }
+    } else {
+        bn = a_dir ? 128 : d.m <= 16 ? 16 : d.m <= 32 ? 32 : d.m <= 64 ? 64 : 128;
+        p.tiles_m = (int)((d.m + bn - 1) / bn); p.tiles_n = (int)((d.n + kRowsX - 1) / kRowsX);
+        p.idesc = f8_idesc(d, true, kRowsX, bn, a_dir, b_dir);
+        const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+        int slices = 1;
+        while (slices < 8 && tiles * slices * 2 <= 2 * g.num_sms && p.num_kb >= slices * 4) slices *= 2;
+        if (o.gemm_fp8_slices > 0) { slices = o.gemm_fp8_slices; while (slices > p.num_kb) slices /= 2; }
+        p.slices = slices;
+        if (tiles * slices > 0x7fffffff) { release(); *err = "too many tiles"; return ACCB_ERR_ARG; }
+    }
+    CUtensorMap ma, mb;
+    if (!make_operand_map(&ma, op[0].base, d.a_type, d.m, d.k, op[0].pitch, pair ? kRowsX : bn, a_dir == 1) ||
+        !make_operand_map(&mb, op[1].base, d.b_type, d.n, d.k, op[1].pitch, kRowsX, b_dir == 1)) {
+        release();
+        *err = "cuTensorMapEncodeTiled failed";
+        return ACCB_ERR_CUDA;
+    }
+    cudaError_t e;
+    if (d.c_type == ACCB_F32) e = launch_c<float>(g, ma, mb, p, bn);
+    else if (d.c_type == ACCB_F16) e = launch_c<__half>(g, ma, mb, p, bn);
+    else e = launch_c<__nv_bfloat16>(g, ma, mb, p, bn);
+    release();
+    if (e != cudaSuccess) { *err = cudaGetErrorString(e); (void)cudaGetLastError(); return ACCB_ERR_CUDA; }
+    note_launches(1);
+    return launches + 1;
+}
+
+}  // namespace accb

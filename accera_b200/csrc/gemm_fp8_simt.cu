@@ -74,7 +74,7 @@ gemm_fp8_simt_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ 
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(part[i][j] * rb[j], ra[i], acc[i][j]);
+            for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(part[i][j], ra[i] * rb[j], acc[i][j]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)

@@ -557,7 +557,7 @@ _FP8_KINDS = {"float8_e4m3fn": E4M3, "float8_e4m3": E4M3, "float8_e5m2": E5M2}
 _TORCH_CODES: dict = {}
 
 
-def _torch_code(dtype):
+def _torch_code(name, dtype):
     if not _TORCH_CODES:
         import torch
         _TORCH_CODES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3,
@@ -565,14 +565,14 @@ def _torch_code(dtype):
     try:
         return _TORCH_CODES[dtype]
     except KeyError:
-        raise TypeError(f"unsupported tensor dtype {dtype}") from None
+        raise TypeError(f"{name}: unsupported tensor dtype {dtype}") from None
 
 
 def _operand(name: str, x, accepted, kind: Optional[str] = None):
     """-> (pointer, element type code, shape, element strides, device index or -1 for host memory) of an array whose type
     is one of `accepted` (type codes).  bf16 and 8-bit floating point numpy arrays are bit patterns (uint16, uint8) that `kind` names."""
     if _is_torch(x):
-        code = _torch_code(x.dtype)
+        code = _torch_code(name, x.dtype)
         if kind is not None and code != _FLOAT_KINDS.get(kind, _FP8_KINDS.get(kind, -1)):
             raise TypeError(f"{name}: a tensor of {x.dtype} is not {kind}")
         desc = x.data_ptr(), code, x.shape, x.stride(), (x.device.index if x.is_cuda else -1)

@@ -294,8 +294,8 @@ int accb_quantize_fp8(const accb_quantize_fp8_desc* desc, const void* x, void* q
  *
  * a_type and b_type are ACCB_E4M3 or ACCB_E5M2, each its own; c_type is ACCB_F32, ACCB_F16 or ACCB_BF16; desc->compute is
  * ACCB_COMPUTE_AUTO, ACCB_COMPUTE_SIMT or ACCB_COMPUTE_TENSOR (which fails where ACCB_COMPUTE_AUTO would take the CUDA
- * cores); max_ctas bounds the persistent grid as for accb_gemm.  Every product of a block and the sum over
- * blocks is accumulated in fp32.
+ * cores); max_ctas > 0 takes the persistent kernel and bounds its grid (rounded up to an even number).  A block's products
+ * and the sum over blocks are accumulated in fp32; the product of a block's two scales is rounded to fp32 first.
  *
  * a_scales is ceil(M / a_block) x ceil(K / 128), b_scales ceil(K / 128) x ceil(N / b_block), a_block and b_block each
  * 1 (a scale per row of A / column of B) or 128, any positive strides; any fp32 value may be a scale.  A product whose
@@ -303,8 +303,8 @@ int accb_quantize_fp8(const accb_quantize_fp8_desc* desc, const void* x, void* q
  * weights' other direction contiguous, the gradient of its input; 1 and 1 is the gradient of its weights.
  *
  * Layouts: on the tensor cores each operand is contiguous along K or along its other direction; C has any strides.
- * Operands whose rows are not 16-byte aligned are copied into aligned rows first, and few-tile problems keep partial
- * sums, both in stream-ordered temporaries of the library.  Host or device pointers as for accb_gemm.
+ * Operands whose rows are not 16-byte aligned are copied into aligned rows first, in a stream-ordered temporary of the
+ * library; nothing else is allocated.  Host or device pointers as for accb_gemm.
  */
 typedef struct accb_fp8_scales {
     int32_t a_block, b_block;        /* 1 or 128 */
@@ -388,6 +388,8 @@ const char* accb_version(void);
  *   "gemm.c_in"              -1 (choose) | 0 | 1      beta != 0 with warp-moved boxes: the old C is copied into the boxes ahead
  *                                                     of its use (1) or read row by row when needed (0)
  *   "gemm.verbose"           0 | 1                    print the launch plan to stderr
+ *   "gemm_fp8.kernel"        0 (choose) | 1 | 2       accb_gemm_fp8: 256 x 256 tiles by CTA pairs (1), 128-column tiles with K slices (2)
+ *   "gemm_fp8.slices"        0 (choose) | 1 | 2 | 4 | 8   K slices of the latter
  *   "stream_kernels.pdl"     -1 (on) | 0 | 1          programmatic dependent launch of the reduce_mean, gather and range kernels
  *   "host_gemm.stage_chunks" 0 (16) | 1..256          row chunks of the staged host-pointer GEMM
  *   "reduce.rows_threads_per_output"  0 (choose) | 32 | 64 | 128 | 256   reduce_mean over contiguous segments

@@ -170,47 +170,60 @@ SHAPES = [(1, 128, 128), (1, 1, 1), (2, 130, 300), (7, 264, 512), (16, 200, 129)
           (65, 129, 48), (100, 256, 1000), (127, 1000, 16), (128, 128, 256), (129, 255, 384), (200, 300, 640), (256, 256, 1152), (300, 520, 4096)]
 
 
-@pytest.mark.parametrize("compute", ["auto", "simt"])
+# every kernel takes every shape: which one runs is a matter of speed alone
+PATHS = {"auto": {}, "simt": {}, "pair": {"gemm_fp8.kernel": 1}, "tile": {"gemm_fp8.kernel": 2, "gemm_fp8.slices": 1},
+         "tile2": {"gemm_fp8.kernel": 2, "gemm_fp8.slices": 2}, "tile8": {"gemm_fp8.kernel": 2, "gemm_fp8.slices": 8}}
+
+
+@pytest.mark.parametrize("path", list(PATHS))
 @pytest.mark.parametrize("ga,gb", [(1, 128), (1, 1), (128, 128), (128, 1)])
 @pytest.mark.parametrize("m,n,k", SHAPES)
-def test_gemm_equals_the_formula(compute, ga, gb, m, n, k):
+def test_gemm_equals_the_formula(path, ga, gb, m, n, k):
     A, sa, B, sb = _operands(m, n, k, "e4m3", "e4m3", ga, gb, m + n + k)
     want, err = _gemm_want(A, sa, B, sb, ga, gb)
-    _check(_run(A, sa, B, sb, ga, gb, "f32", compute=compute), want, err, (compute, ga, gb))
+    with rt.options(**PATHS[path]):
+        got = _run(A, sa, B, sb, ga, gb, "f32", compute="simt" if path == "simt" else "tensor" if path != "auto" else "auto")
+    _check(got, want, err, (path, ga, gb))
 
 
 @pytest.mark.parametrize("a,b", [("e4m3", "e4m3"), ("e5m2", "e4m3"), ("e4m3", "e5m2"), ("e5m2", "e5m2")])
 @pytest.mark.parametrize("c", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("layout", ["tn", "tt", "nn", "nt"])
-@pytest.mark.parametrize("m,n,k", [(9, 144, 272), (272, 400, 528), (144, 272, 1040)])
-def test_gemm_types_and_layouts(a, b, c, layout, m, n, k):
+@pytest.mark.parametrize("path,m,n,k", [("tile", 9, 144, 272), ("tile8", 144, 272, 1040), ("pair", 272, 400, 528)])
+def test_gemm_types_and_layouts(a, b, c, layout, path, m, n, k):
     A, sa, B, sb = _operands(m, n, k, a, b, 1, 128, 3)
     sb *= 0.001                                                        # inside fp16's range
     want, err = _gemm_want(A, sa, B, sb, 1, 128)
     assert want.abs().max() < 60000
-    _check(_run(A, sa, B, sb, 1, 128, c, layout), want, err, (a, b, c, layout))
+    with rt.options(**PATHS[path]):
+        got = _run(A, sa, B, sb, 1, 128, c, layout, compute="tensor")
+    _check(got, want, err, (a, b, c, layout))
 
 
 @pytest.mark.parametrize("alpha,beta,relu,use_bias", [(1.0, 1.0, False, False), (0.5, 0.0, True, True), (-2.0, 0.25, False, True), (1.0, 1.0, True, True)])
 @pytest.mark.parametrize("c", ["f32", "bf16"])
-@pytest.mark.parametrize("m,n,k", [(1, 256, 512), (40, 200, 300), (200, 264, 768), (520, 512, 256)])
-def test_gemm_epilogue(alpha, beta, relu, use_bias, c, m, n, k):
+@pytest.mark.parametrize("path", ["pair", "tile", "tile8", "simt"])
+@pytest.mark.parametrize("m,n,k", [(1, 256, 512), (40, 203, 300), (200, 264, 768), (520, 512, 256)])
+def test_gemm_epilogue(alpha, beta, relu, use_bias, c, path, m, n, k):
     A, sa, B, sb = _operands(m, n, k, "e4m3", "e4m3", 1, 128, 4)
     old = (torch.randn(m, n) * 100).to(TYPES[c])
     bias = torch.randn(n) * 100 if use_bias else None
     want, err = _gemm_want(A, sa, B, sb, 1, 128, old, alpha, beta, bias, relu)
-    _check(_run(A, sa, B, sb, 1, 128, c, old=old, alpha=alpha, beta=beta, relu=relu, bias=bias), want, err, "epilogue")
+    with rt.options(**PATHS[path]):
+        got = _run(A, sa, B, sb, 1, 128, c, old=old, alpha=alpha, beta=beta, relu=relu, bias=bias, compute="simt" if path == "simt" else "auto")
+    _check(got, want, err, "epilogue")
 
 
-@pytest.mark.parametrize("m,n,k", [(3, 130, 256), (200, 300, 384)])
-def test_gemm_result_strides_leave_the_rest_alone(m, n, k):
+@pytest.mark.parametrize("path,m,n,k", [("tile", 3, 130, 256), ("tile2", 200, 300, 384), ("pair", 200, 300, 384)])
+def test_gemm_result_strides_leave_the_rest_alone(path, m, n, k):
     A, sa, B, sb = _operands(m, n, k, "e4m3", "e4m3", 1, 128, 5)
     want, err = _gemm_want(A, sa, B, sb, 1, 128)
     for make in (lambda: torch.full((m, n + 5), 7.0, device="cuda")[:, 2:n + 2], lambda: torch.full((n + 3, m + 1), 7.0, device="cuda")[1:n + 1, :m].t(),
                  lambda: torch.full((m, 2 * n), 7.0, device="cuda")[:, ::2]):
         C = make()
         base = C._base if C._base is not None else C
-        rt.gemm_fp8(A.cuda(), B.cuda().t(), C, sa.cuda(), sb.cuda().t(), beta=0.0)
+        with rt.options(**PATHS[path]):
+            rt.gemm_fp8(A.cuda(), B.cuda().t(), C, sa.cuda(), sb.cuda().t(), beta=0.0)
         rt.synchronize()
         _check(C.cpu(), want, err, tuple(C.stride()))
         left = base.clone()
@@ -254,7 +267,13 @@ def test_gemm_empty_k_and_special_scales():
     sa[9, 1] = float("inf")
     sa[20, 0] = 0.0
     sb[17, 2] = float("nan")
-    got = _run(A, sa, B, sb, 1, 1, "f32")
+    for path in PATHS:
+        with rt.options(**PATHS[path]):
+            got = _run(A, sa, B, sb, 1, 1, "f32", compute="simt" if path == "simt" else "auto")
+        _check_broken(got, m, n)
+
+
+def _check_broken(got, m, n):
     broken = torch.zeros(m, n, dtype=torch.bool)
     broken[3] = broken[9] = True
     broken[:, 17] = True
