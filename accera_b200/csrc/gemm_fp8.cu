@@ -9,8 +9,11 @@
 //
 // Two kernels:
 //   pair   256 x 256 tiles by CTA pairs (cta_group::2), persistent: every SM multiplies 128 x 256 x 128 a block, in
-//          512 cycles at the nominal 8-bit rate.  Eight epilogue warps hold the sums, 128 fp32 a thread, and spend 64 packed
-//          fused multiply-adds a thread a block on them: two warps a scheduler, about half of its issue slots.
+//          512 cycles at the nominal 8-bit rate.  Eight epilogue warps hold the sums, 128 fp32 a thread; while a warp adds
+//          32 columns the next 32 are on their way from TMEM.  8192^3, e4m3 to bf16: 550 us (2.0 PFLOP/s); the same loads and
+//          MMAs without the additions take 397 us, so the loop is bound by the round trip of a TMEM buffer (MMAs done -
+//          read by both CTAs' warps - MMA issued again), of which only two fit TMEM at this width.  Narrower tiles with
+//          three or four buffers (160, 128 columns) were measured slower, 650 and 700 us: their operands alone take 500 and 540.
 //   tile   128 x BN tiles by single CTAs for problems with too few large tiles: columns of C (weights) on the 128 TMEM
 //          lanes, rows of C (tokens) on BN = 16 .. 128 accumulator columns, K cut into up to eight slices
 //          that a cluster multiplies side by side and adds, slice by slice, through distributed shared memory.
@@ -27,6 +30,7 @@
 #include <type_traits>
 
 #include "accb_internal.h"
+#define ACCB_WAIT_INLINE __forceinline__
 #include "umma_device.h"
 
 namespace accb {
@@ -116,6 +120,19 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar)
 {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// Arrival on a barrier of the pair's rank 0 that only says "these TMEM columns have been read" (tcgen05.wait::ld and
+// tcgen05.fence::before_thread_sync come before it): no memory of this thread needs to be visible with it.
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank)
 {
     uint32_t r;
@@ -128,6 +145,36 @@ __device__ __forceinline__ float load_cluster(uint32_t addr)
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
+
+// Four tcgen05.mma that multiply one stage (128 bytes of K a row) into a fresh accumulator, issued by the elected lane of
+// a warp that runs converged, so that descriptors stay in uniform registers.  *_step: what 32 bytes of K add to a descriptor.
+template <bool PAIR>
+__device__ __forceinline__ void mma_block(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t a_step, uint32_t b_step, uint32_t elected)
+{
+#define ACCB_F8_MMA(GROUP, A, B, ADD) "@e tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], " A ", " B ", %3, " ADD ";\n\t"
+#define ACCB_F8_BLOCK(GROUP)                                                                                          \
+    asm volatile("{\n\t.reg .pred e, fresh, add;\n\t.reg .b64 as, bs, a1, a2, a3, b1, b2, b3;\n\t"                   \
+                 "setp.ne.b32 e, %6, 0;\n\tsetp.ne.b32 fresh, 0, 0;\n\tsetp.eq.b32 add, 0, 0;\n\t"                   \
+                 "cvt.u64.u32 as, %4;\n\tcvt.u64.u32 bs, %5;\n\t"                                                    \
+                 "add.u64 a1, %1, as;\n\tadd.u64 b1, %2, bs;\n\tadd.u64 a2, a1, as;\n\tadd.u64 b2, b1, bs;\n\t"      \
+                 "add.u64 a3, a2, as;\n\tadd.u64 b3, b2, bs;\n\t"                                                    \
+                 ACCB_F8_MMA(GROUP, "%1", "%2", "fresh") ACCB_F8_MMA(GROUP, "a1", "b1", "add")                        \
+                 ACCB_F8_MMA(GROUP, "a2", "b2", "add") ACCB_F8_MMA(GROUP, "a3", "b3", "add") "}"                      \
+                 ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(a_step), "r"(b_step), "r"(elected) : "memory")
+    if constexpr (PAIR) ACCB_F8_BLOCK("2");
+    else ACCB_F8_BLOCK("1");
+#undef ACCB_F8_BLOCK
+#undef ACCB_F8_MMA
+}
+__device__ __forceinline__ uint32_t elect_lane()
+{
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e;
+}
+// operand descriptor of the ring's first stage, and what 32 bytes of K add to it
+__device__ __forceinline__ uint64_t operand_desc(uint32_t smem, int mn) { return mn ? make_smem_desc_mn(smem, kSlabBytes * kSlabBytes) : make_smem_desc(smem); }
+__device__ __forceinline__ uint32_t operand_step(int mn) { return (uint32_t)((mn ? kMmaKBytes * kSlabBytes : kMmaKBytes) >> 4); }
 
 // alpha, beta * old, bias and ReLU of one value; a NaN stays NaN
 __device__ __forceinline__ float finish(float acc, float old, float bias, const F8Params& p)
@@ -144,7 +191,12 @@ __device__ __forceinline__ float finish(float acc, float old, float bias, const 
 // ---------------------------------------------------------------------------------
 
 struct PairPlan {
-    static constexpr int kThreads = 320;                                // TMA + scales, MMA, eight epilogue warps
+    static constexpr int kThreads = 384;                                // TMA, MMA, scales, an idle warp; eight epilogue warps
+    static constexpr int kEpilogueWarp = 4;                             // first of them
+    // Registers a thread: the launch gets 65536 / 384, rounded down to 168; the epilogue warps, with 128 sums and 64 values on
+    // their way from TMEM, take what the first four warps give up: 4 * 40 + 8 * 232 = 12 * 168
+    static constexpr int kFewRegisters = 40, kManyRegisters = 232;
+    static constexpr int kGroup = 4, kSlots = 4;                        // scales: blocks a ring slot, slots
     static constexpr int kBN = 256;
     static constexpr int kStageBytes = 2 * kRowsX * kSlabBytes;         // 16 KB of A, 16 KB of B (this CTA's half of the columns)
     static constexpr int kStages = 5;
@@ -152,7 +204,7 @@ struct PairPlan {
     static constexpr int kScaleBytes = (kRowsX + kBN) * 4;
     static constexpr int kBoxes = kStages * kStageBytes;
     static constexpr int kScales = kBoxes + 8 * kBoxBytes;
-    static constexpr int kBars = kScales + kRing * kScaleBytes;
+    static constexpr int kBars = kScales + kSlots * kGroup * kScaleBytes;
     static constexpr int kTotal = kBars + 512 + 1024;                   // + manual alignment
     static_assert(kTotal <= 227 * 1024, "shared memory of a CTA");
 };
@@ -163,56 +215,79 @@ template <typename TC>
 __device__ __forceinline__ void store_box(float (&v)[128 / sizeof(TC)], uint8_t* box, TC* C, int64_t row0, int64_t col0, int lane, const F8Params& p)
 {
     constexpr int W = 128 / (int)sizeof(TC), V = 16 / (int)sizeof(TC);
-    if (p.c_mode == 0) {
-        const int64_t row = row0 + lane;
-        if (row < p.m) {
+    const int cols = (int)(p.n - col0 < W ? p.n - col0 : W), rows = (int)(p.m - row0 < 32 ? p.m - row0 : 32);
+    if (p.alpha != 1.0f) {
 #pragma unroll
-            for (int j = 0; j < W; ++j)
-                if (col0 + j < p.n) {
-                    TC* d = C + row * p.cs0 + (col0 + j) * p.cs1;
-                    *d = (TC)finish(v[j], p.beta != 0.0f ? (float)*d : 0.0f, p.bias ? __ldg(p.bias + col0 + j) : 0.0f, p);
-                }
+        for (int j = 0; j < W; ++j) v[j] *= p.alpha;
+    }
+    if (p.c_mode == 0) {
+        if (lane < rows) {
+            TC* d = C + (row0 + lane) * p.cs0 + col0 * p.cs1;
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                if (j >= cols) break;
+                float x = v[j];
+                if (p.beta != 0.0f) x = fmaf(p.beta, (float)d[j * p.cs1], x);
+                if (p.bias) x += __ldg(p.bias + col0 + j);
+                if (p.relu) x = x < 0.0f ? 0.0f : x;
+                d[j * p.cs1] = (TC)x;
+            }
         }
         return;
     }
-    const bool vec = p.c_mode == 2;
-    auto slot_of = [&](int r, int s) { return box + r * 128 + ((s ^ (r & 7)) << 4); };
+    // along rows: lane / 8 is one of four rows, lane % 8 a slot; `base` addresses that lane's 16 bytes of the first four rows
+    const int r0 = lane >> 3, slot = lane & 7;
+    TC* base = C + (row0 + r0) * p.cs0 + col0 + slot * V;
+    const int in_slot = cols - slot * V;                     // elements of the lane's slot inside the matrix
+    const bool vec = p.c_mode == 2 && in_slot >= V;
+    uint8_t* own = box + lane * 128;                         // this thread's row; its slots are at s ^ (lane & 7)
+    const int flip = (lane & 7) << 4;
     if (p.beta != 0.0f) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + lane / 8, s = lane % 8;
-            const int64_t col = col0 + s * V;
-            if (row0 + r >= p.m || col >= p.n) continue;
-            const TC* src = C + (row0 + r) * p.cs0 + col;
-            if (vec && col + V <= p.n) *reinterpret_cast<uint4*>(slot_of(r, s)) = *reinterpret_cast<const uint4*>(src);
+            const int r = i * 4 + r0;
+            uint8_t* at = box + r * 128 + ((slot ^ (r & 7)) << 4);
+            const TC* src = base + (int64_t)(i * 4) * p.cs0;
+            if (r >= rows) continue;
+            if (vec) *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(src);
             else
-                for (int e = 0; e < V; ++e) if (col + e < p.n) reinterpret_cast<TC*>(slot_of(r, s))[e] = src[e];
+                for (int e = 0; e < V && e < in_slot; ++e) reinterpret_cast<TC*>(at)[e] = src[e];
         }
         __syncwarp();
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            const uint4 w = *reinterpret_cast<const uint4*>(own + ((s << 4) ^ flip));
+            const TC* h = reinterpret_cast<const TC*>(&w);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[s * V + e] = fmaf(p.beta, (float)h[e], v[s * V + e]);
+        }
+    }
+    if (p.bias) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[j] += j < cols ? __ldg(p.bias + col0 + j) : 0.0f;
+    }
+    if (p.relu) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];
     }
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        uint8_t* own = slot_of(lane, s);
-        if (p.beta != 0.0f) w = *reinterpret_cast<const uint4*>(own);
+        uint4 w;
         TC* h = reinterpret_cast<TC*>(&w);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const int64_t col = col0 + s * V + e;
-            h[e] = (TC)finish(v[s * V + e], (float)h[e], p.bias && col < p.n ? __ldg(p.bias + col) : 0.0f, p);
-        }
-        *reinterpret_cast<uint4*>(own) = w;
+        for (int e = 0; e < V; ++e) h[e] = (TC)v[s * V + e];
+        *reinterpret_cast<uint4*>(own + ((s << 4) ^ flip)) = w;
     }
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int r = i * 4 + lane / 8, s = lane % 8;
-        const int64_t col = col0 + s * V;
-        if (row0 + r >= p.m || col >= p.n) continue;
-        TC* dst = C + (row0 + r) * p.cs0 + col;
-        if (vec && col + V <= p.n) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(slot_of(r, s));
+        const int r = i * 4 + r0;
+        const uint8_t* at = box + r * 128 + ((slot ^ (r & 7)) << 4);
+        TC* dst = base + (int64_t)(i * 4) * p.cs0;
+        if (r >= rows) continue;
+        if (vec) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(at);
         else
-            for (int e = 0; e < V; ++e) if (col + e < p.n) dst[e] = reinterpret_cast<const TC*>(slot_of(r, s))[e];
+            for (int e = 0; e < V && e < in_slot; ++e) dst[e] = reinterpret_cast<const TC*>(at)[e];
     }
     __syncwarp();
 }
@@ -228,6 +303,23 @@ __device__ __forceinline__ void pair_tile(int t, const F8Params& p, int& tm, int
     tn = in / rows;
 }
 
+// 32 columns of a block's product, times the product of the scales, to the sums: one scale for all, or one for each column
+__device__ __forceinline__ void add_scaled(float* acc, const uint32_t (&x)[32], float f)
+{
+#pragma unroll
+    for (int j = 0; j < 32; ++j) acc[j] = fmaf(__uint_as_float(x[j]), f, acc[j]);
+}
+__device__ __forceinline__ void add_scaled(float* acc, const uint32_t (&x)[32], float f, const float4 (&w)[8])
+{
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        acc[4 * j] = fmaf(__uint_as_float(x[4 * j]), f * w[j].x, acc[4 * j]);
+        acc[4 * j + 1] = fmaf(__uint_as_float(x[4 * j + 1]), f * w[j].y, acc[4 * j + 1]);
+        acc[4 * j + 2] = fmaf(__uint_as_float(x[4 * j + 2]), f * w[j].z, acc[4 * j + 2]);
+        acc[4 * j + 3] = fmaf(__uint_as_float(x[4 * j + 3]), f * w[j].w, acc[4 * j + 3]);
+    }
+}
+
 // COLS: every column of B has a scale of its own (else 128 share one)
 template <typename TC, bool COLS>
 __global__ void __launch_bounds__(PairPlan::kThreads, 1)
@@ -240,12 +332,13 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t bars = smem_base + Plan::kBars;
     auto full_bar = [&](int s) { return bars + 8u * s; };
-    auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
-    auto tmem_full_bar = [&](int b) { return bars + 8u * (2 * S + b); };
-    auto tmem_empty_bar = [&](int b) { return bars + 8u * (2 * S + 2 + b); };
-    auto scale_full_bar = [&](int r) { return bars + 8u * (2 * S + 4 + r); };
-    auto scale_empty_bar = [&](int r) { return bars + 8u * (2 * S + 4 + kRing + r); };
-    volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(smem_gen + Plan::kBars + 8 * (2 * S + 4 + 2 * kRing));
+    // A block's MMAs are complete: its stage may be loaded again and its accumulator read.  One commit a block for both,
+    // because the issuing thread pays for each; neither side can be a whole turn of the ring behind.
+    auto done_bar = [&](int s) { return bars + 8u * (S + s); };
+    auto tmem_empty_bar = [&](int b) { return bars + 8u * (2 * S + b); };
+    auto scale_full_bar = [&](int r) { return bars + 8u * (2 * S + 2 + r); };
+    auto scale_empty_bar = [&](int r) { return bars + 8u * (2 * S + 2 + Plan::kSlots + r); };
+    volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(smem_gen + Plan::kBars + 8 * (2 * S + 2 + 2 * Plan::kSlots));
     volatile uint32_t* gave_up = tmem_holder + 2;        // one word a CTA of the pair, each CTA with a copy of both
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -263,9 +356,9 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         gave_up[1] = 0u;
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_a)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_b)) : "memory");
-        for (int s = 0; s < S; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(tmem_full_bar(b), 1); mbar_init(tmem_empty_bar(b), 16); }   // a commit; the warps of both CTAs
-        for (int r = 0; r < kRing; ++r) { mbar_init(scale_full_bar(r), 32); mbar_init(scale_empty_bar(r), 8); }
+        for (int s = 0; s < S; ++s) { mbar_init(full_bar(s), 1); mbar_init(done_bar(s), 1); }
+        for (int b = 0; b < 2; ++b) mbar_init(tmem_empty_bar(b), 16);                          // the epilogue warps of both CTAs
+        for (int r = 0; r < Plan::kSlots; ++r) { mbar_init(scale_full_bar(r), 32); mbar_init(scale_empty_bar(r), 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -282,145 +375,168 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     const int num_units = (int)gridDim.x / 2, unit = (int)blockIdx.x / 2;
     const int num_kb = p.num_kb;
 
+    if (warp < Plan::kEpilogueWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Plan::kFewRegisters));
     if (warp == 0) {
-        // ---------------- scales by the whole warp, TMA loads by lane 0 ----------------
-        int s = 0, r = 0;
-        uint32_t ph = 0, rph = 0;
+        // ---------------- TMA producer ----------------
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int t = unit; t < num_tiles && ok; t += num_units) {
+                int tm, tn;
+                pair_tile(t, p, tm, tn);
+                const int row_a = (tm * 2 + (int)rank) * kRowsX, row_b = tn * Plan::kBN + (int)rank * 128;
+                for (int kb = 0; kb < num_kb; ++kb) {
+                    if (!mbar_wait(done_bar(s), ph ^ 1u, wctx, SITE_PRODUCER_EMPTY, kb)) { ok = false; break; }
+                    const uint32_t sa = smem_base + s * Plan::kStageBytes, sb = sa + kRowsX * kSlabBytes;
+                    if (leader) mbar_arrive_expect_tx(full_bar(s), 2u * Plan::kStageBytes);
+                    if (p.a_mn) tma_load_2d_pair(sa, &map_a, full_bar(s), row_a, kb * kSlabBytes, 0);
+                    else tma_load_2d_pair(sa, &map_a, full_bar(s), kb * kSlabBytes, row_a, 0);
+                    if (p.b_mn) tma_load_2d_pair(sb, &map_b, full_bar(s), row_b, kb * kSlabBytes, 0);
+                    else tma_load_2d_pair(sb, &map_b, full_bar(s), kb * kSlabBytes, row_b, 0);
+                    if (++s == S) { s = 0; ph ^= 1u; }
+                }
+            }
+            if (!ok) record_give_up();
+        }
+    } else if (warp == 2) {
+        // ---------------- scales ----------------
+        int r = 0;
+        uint32_t rph = 0;
         bool ok = true;
         for (int t = unit; t < num_tiles && ok; t += num_units) {
             int tm, tn;
             pair_tile(t, p, tm, tn);
-            const int row_a = (tm * 2 + (int)rank) * kRowsX, col_b = tn * Plan::kBN, row_b = col_b + (int)rank * 128;
-            const float* src_a[4];
-            bool in_a[4];
+            const int64_t row_a = (int64_t)(tm * 2 + (int)rank) * kRowsX + lane, col_b = (int64_t)tn * Plan::kBN + lane * (COLS ? 1 : 128);
+            for (int kb0 = 0; kb0 < num_kb; kb0 += Plan::kGroup) {
+                ok = __all_sync(0xffffffffu, mbar_wait(scale_empty_bar(r), rph ^ 1u, wctx, SITE_PRODUCER_EMPTY, kb0));
+                if (!ok) break;
+                const int blocks = min(Plan::kGroup, num_kb - kb0);
+                for (int j = 0; j < blocks; ++j) {
+                    const uint32_t sc = smem_base + Plan::kScales + (r * Plan::kGroup + j) * Plan::kScaleBytes;
+                    const float* sa = p.sa + (kb0 + j) * p.sa_kb;
+                    const float* sb = p.sb + (kb0 + j) * p.sb_kb;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int64_t row = row_a + i * 32 + lane;
-                in_a[i] = row < p.m;
-                src_a[i] = p.sa + (in_a[i] ? (row >> p.a_shift) * p.sa_row : 0);
-            }
-            constexpr int kColLoads = COLS ? 8 : 1;
-            const float* src_b[kColLoads];
-            bool in_b[kColLoads];
+                    for (int i = 0; i < 4; ++i) {
+                        const int64_t row = row_a + i * 32;
+                        copy_scale(sc + (i * 32 + lane) * 4, sa + (row < p.m ? (row >> p.a_shift) * p.sa_row : 0), row < p.m);
+                    }
 #pragma unroll
-            for (int i = 0; i < kColLoads; ++i) {
-                const int64_t col = COLS ? (int64_t)col_b + i * 32 + lane : (int64_t)col_b + lane * 128;
-                in_b[i] = col < p.n && (COLS || lane < 2);
-                src_b[i] = p.sb + (in_b[i] ? (col >> p.b_shift) * p.sb_col : 0);
-            }
-            for (int kb = 0; kb < num_kb; ++kb) {
-                ok = mbar_wait(scale_empty_bar(r), rph ^ 1u, wctx, SITE_PRODUCER_EMPTY, kb);
-                if (ok) {
-                    const uint32_t sc = smem_base + Plan::kScales + r * Plan::kScaleBytes;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) copy_scale(sc + (i * 32 + lane) * 4, src_a[i] + kb * p.sa_kb, in_a[i]);
-#pragma unroll
-                    for (int i = 0; i < kColLoads; ++i)
-                        if (COLS || lane < 2) copy_scale(sc + (kRowsX + i * 32 + lane) * 4, src_b[i] + kb * p.sb_kb, in_b[i]);
-                    copies_arrive(scale_full_bar(r));
-                    if (++r == kRing) { r = 0; rph ^= 1u; }
-                }
-                if (lane == 0 && ok) {
-                    ok = mbar_wait(empty_bar(s), ph ^ 1u, wctx, SITE_PRODUCER_EMPTY, kb);
-                    if (ok) {
-                        const uint32_t sa = smem_base + s * Plan::kStageBytes, sb = sa + kRowsX * kSlabBytes;
-                        if (leader) mbar_arrive_expect_tx(full_bar(s), 2u * Plan::kStageBytes);
-                        if (p.a_mn) tma_load_2d_pair(sa, &map_a, full_bar(s), row_a, kb * kSlabBytes, 0);
-                        else tma_load_2d_pair(sa, &map_a, full_bar(s), kb * kSlabBytes, row_a, 0);
-                        if (p.b_mn) tma_load_2d_pair(sb, &map_b, full_bar(s), row_b, kb * kSlabBytes, 0);
-                        else tma_load_2d_pair(sb, &map_b, full_bar(s), kb * kSlabBytes, row_b, 0);
+                    for (int i = 0; i < (COLS ? 8 : 1); ++i) {
+                        const int64_t col = col_b + i * 32;
+                        if (COLS || lane < 2) copy_scale(sc + (kRowsX + i * 32 + lane) * 4, sb + (col < p.n ? (col >> p.b_shift) * p.sb_col : 0), col < p.n);
                     }
                 }
-                if (++s == S) { s = 0; ph ^= 1u; }
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                copies_arrive(scale_full_bar(r));
+                if (++r == Plan::kSlots) { r = 0; rph ^= 1u; }
             }
         }
         if (!ok && lane == 0) record_give_up();
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == 1) {
         // ---------------- MMA issuer (rank 0 of the pair) ----------------
-        if (lane == 0 && leader) {
-            auto issue = [&](auto a_mn_tag, auto b_mn_tag) {
-                constexpr bool A_MN = decltype(a_mn_tag)::value, B_MN = decltype(b_mn_tag)::value;
-                int s = 0, g = 0;
-                uint32_t ph = 0;
-                bool ok = true;
-                for (int t = unit; t < num_tiles && ok; t += num_units) {
-                    for (int kb = 0; kb < num_kb; ++kb, ++g) {
-                        const int buf = g & 1;
-                        if (!mbar_wait(tmem_empty_bar(buf), ((g >> 1) & 1u) ^ 1u, wctx, SITE_MMA_TMEM_EMPTY, kb) ||
-                            !mbar_wait(full_bar(s), ph, wctx, SITE_MMA_FULL, kb)) { ok = false; break; }
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t sa = smem_base + s * Plan::kStageBytes;
-                        issue_stage<KIND_F8F6F4, true, A_MN, B_MN>(tmem_base + (uint32_t)(buf * Plan::kBN), sa, sa + kRowsX * kSlabBytes, p.idesc, true);
-                        umma_commit<true>(empty_bar(s));
-                        umma_commit<true>(tmem_full_bar(buf));
-                        if (++s == S) { s = 0; ph ^= 1u; }
-                    }
-                }
-                if (!ok) record_give_up();
-            };
-            if (!p.a_mn && !p.b_mn) issue(std::false_type{}, std::false_type{});
-            else if (!p.b_mn) issue(std::true_type{}, std::false_type{});
-            else if (!p.a_mn) issue(std::false_type{}, std::true_type{});
-            else issue(std::true_type{}, std::true_type{});
+        if (leader) {
+            const uint64_t a0 = operand_desc(smem_base, p.a_mn), b0 = operand_desc(smem_base + kRowsX * kSlabBytes, p.b_mn);
+            const uint32_t a_step = operand_step(p.a_mn), b_step = operand_step(p.b_mn), elected = elect_lane();
+            const int blocks = (num_tiles - unit + num_units - 1) / num_units * num_kb;
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int g = 0; g < blocks; ++g) {
+                ok = mbar_wait(full_bar(s), ph, wctx, SITE_MMA_FULL, g) &&
+                     mbar_wait(tmem_empty_bar(g & 1), ((g >> 1) & 1u) ^ 1u, wctx, SITE_MMA_TMEM_EMPTY, g);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t stage = (uint64_t)(s * (Plan::kStageBytes >> 4));
+                mma_block<true>(tmem_base + (uint32_t)((g & 1) * Plan::kBN), a0 + stage, b0 + stage, p.idesc, a_step, b_step, elected);
+                if (elected) umma_commit<true>(done_bar(s));
+                __syncwarp();
+                if (++s == S) { s = 0; ph ^= 1u; }
+            }
+            if (!ok && lane == 0) record_give_up();
         }
+    }
     } else {
         // ---------------- epilogue warps ----------------
-        const int q = warp & 3, ew = warp - 2, half = ew >> 2;      // TMEM lane quarter, half of the tile's columns
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Plan::kManyRegisters));
+        const int q = warp & 3, ew = warp - Plan::kEpilogueWarp, half = ew >> 2;     // TMEM lane quarter, half of the tile's columns
         uint8_t* box = smem_gen + Plan::kBoxes + ew * Plan::kBoxBytes;
         const float* scales = reinterpret_cast<const float*>(smem_gen + Plan::kScales);
         const uint32_t taddr0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
-        int g = 0, r = 0;
-        uint32_t rph = 0;
+        int g = 0, r = 0, s = 0;
+        uint32_t rph = 0, ph = 0;
         bool ok = true;
         for (int t = unit; t < num_tiles && ok; t += num_units) {
             int tm, tn;
             pair_tile(t, p, tm, tn);
-            uint64_t acc[64];
+            float acc[128];
 #pragma unroll
-            for (int i = 0; i < 64; ++i) acc[i] = 0ull;
+            for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
+            // One load of 32 columns is always on its way while the 32 before it are added: the first of a block is issued
+            // before the last of the block before it is added, if that block's MMAs are done by then.
+            uint32_t x0[32], x1[32];
+            bool loading = false;
             for (int kb = 0; kb < num_kb; ++kb, ++g) {
-                const int buf = g & 1;
-                ok = mbar_wait(scale_full_bar(r), rph, wctx, SITE_EPI_TMEM_FULL, kb) &&
-                     mbar_wait(tmem_full_bar(buf), (g >> 1) & 1u, wctx, SITE_EPI_TMEM_FULL, kb);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const float* sc = scales + r * (Plan::kScaleBytes / 4);
-                const float row_scale = sc[q * 32 + lane];
-                const float* col_scale = sc + kRowsX + (COLS ? half * 128 : half);
-                const float f = COLS ? row_scale : row_scale * col_scale[0];
-                const uint64_t f2 = pack2(__float_as_uint(f), __float_as_uint(f));
+                const int buf = g & 1, in_group = kb % Plan::kGroup;
                 const uint32_t taddr = taddr0 + (uint32_t)(buf * Plan::kBN);
-                uint32_t x[2][16];
-                tmem_ld16(taddr, x[0]);
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    tmem_wait_ld16(x[c & 1]);
-                    if (c < 7) tmem_ld16(taddr + (uint32_t)(16 * (c + 1)), x[(c + 1) & 1]);
-                    else {
-                        // this warp has read the buffer: the MMA issuer of the pair may overwrite it
-                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(tmem_empty_bar(buf) & kPeerMask);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
-                        uint64_t g0 = f2, g1 = f2;
-                        if constexpr (COLS) {
-                            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(col_scale + 16 * c + 2 * j);
-                            g0 = mul2(f2, w.x);
-                            g1 = mul2(f2, w.y);
-                        }
-                        acc[8 * c + j] = fma2(pack2(x[c & 1][2 * j], x[c & 1][2 * j + 1]), g0, acc[8 * c + j]);
-                        acc[8 * c + j + 1] = fma2(pack2(x[c & 1][2 * j + 2], x[c & 1][2 * j + 3]), g1, acc[8 * c + j + 1]);
-                    }
+                if (in_group == 0) ok = mbar_wait(scale_full_bar(r), rph, wctx, SITE_EPI_TMEM_FULL, kb);
+                if (!loading) {
+                    ok = ok && mbar_wait(done_bar(s), ph, wctx, SITE_EPI_TMEM_FULL, kb);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    tmem_ld32(taddr, x0);
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(scale_empty_bar(r));
-                if (++r == kRing) { r = 0; rph ^= 1u; }
+                if (++s == S) { s = 0; ph ^= 1u; }
+                const float* sc = scales + (r * Plan::kGroup + in_group) * (Plan::kScaleBytes / 4);
+                const float* col_scale = sc + kRowsX + (COLS ? half * 128 : half);
+                if constexpr (COLS) {
+                    // the columns' scales need the registers of a second load: they are read while the one load is on its way
+                    const float f = sc[q * 32 + lane];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float4 w[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) w[j] = *reinterpret_cast<const float4*>(col_scale + 32 * c + 4 * j);
+                        tmem_wait_ld(x0);
+                        if (c == 3) {
+                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive_pair(tmem_empty_bar(buf) & kPeerMask);
+                        }
+                        add_scaled(acc + 32 * c, x0, f, w);
+                        if (c < 3) tmem_ld32(taddr + 32 * (c + 1), x0);
+                    }
+                } else {
+                    const float f = sc[q * 32 + lane] * col_scale[0];
+                    tmem_wait_ld(x0);
+                    tmem_ld32(taddr + 32, x1);
+                    add_scaled(acc, x0, f);
+                    tmem_wait_ld(x1);
+                    tmem_ld32(taddr + 64, x0);
+                    add_scaled(acc + 32, x1, f);
+                    tmem_wait_ld(x0);
+                    tmem_ld32(taddr + 96, x1);
+                    const bool next = kb + 1 < num_kb && mbar_test(done_bar(s), ph);
+                    add_scaled(acc + 64, x0, f);
+                    tmem_wait_ld(x1);
+                    // this warp has read the buffer: the MMA issuer of the pair may overwrite it
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    loading = __all_sync(0xffffffffu, next);
+                    if (lane == 0) mbar_arrive_pair(tmem_empty_bar(buf) & kPeerMask);
+                    if (loading) {
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        tmem_ld32(taddr0 + (uint32_t)((buf ^ 1) * Plan::kBN), x0);
+                    }
+                    add_scaled(acc + 96, x1, f);
+                }
+                if (in_group == Plan::kGroup - 1 || kb == num_kb - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(scale_empty_bar(r));
+                    if (++r == Plan::kSlots) { r = 0; rph ^= 1u; }
+                }
             }
             if (!ok) break;
             const int64_t row0 = (int64_t)(tm * 2 + (int)rank) * kRowsX + q * 32, col0 = (int64_t)tn * Plan::kBN + half * 128;
@@ -429,7 +545,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             for (int b = 0; b < 128 / W; ++b) {
                 float v[W];
 #pragma unroll
-                for (int j = 0; j < W; j += 2) unpack2(acc[(b * W + j) / 2], v[j], v[j + 1]);
+                for (int j = 0; j < W; ++j) v[j] = acc[b * W + j];
                 if (row0 < p.m && col0 + b * W < p.n) store_box<TC>(v, box, C, row0, col0 + b * W, lane, p);
             }
         }

@@ -53,10 +53,16 @@ __device__ __forceinline__ unsigned long long global_timer_ns()
     return t;
 }
 
+// ACCB_WAIT_INLINE: how a file takes the waiting loop.  Out of line keeps the code small; a kernel that moves registers
+// between its warps (setmaxnreg) must not contain calls.
+#ifndef ACCB_WAIT_INLINE
+#define ACCB_WAIT_INLINE __noinline__
+#endif
+
 // Bounded wait.  Returns false when it gave up: after `wait_ns` (a second unless the caller asked otherwise), or as
 // soon as a CTA of THIS launch has recorded a failure.  The first failure of a launch is recorded with the launch's
 // id; a record left by an earlier launch is not this launch's business and neither stops it nor is overwritten.
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, int* status, int launch_id, unsigned long long wait_ns,
+__device__ ACCB_WAIT_INLINE bool mbar_wait_slow(uint32_t bar, uint32_t parity, int* status, int launch_id, unsigned long long wait_ns,
                                             int site, int detail)
 {
     const unsigned long long t0 = global_timer_ns();
@@ -78,7 +84,7 @@ __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, int* 
 struct WaitCtx { int* status; int launch_id; unsigned long long wait_ns; };
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const WaitCtx& w, int site, int detail)
 {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
     return mbar_wait_slow(bar, parity, w.status, w.launch_id, w.wait_ns, site, detail);
 }
 

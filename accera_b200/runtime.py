@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Optional
 
 import numpy as np
@@ -115,13 +116,13 @@ def lib() -> ctypes.CDLL:
     L.accb_gather_rank2.restype = ctypes.c_int
     L.accb_gather_rank2_dims.argtypes = [i64, i64, i64, i64, i32, ctypes.POINTER(i64)]
     L.accb_gather_rank2_dims.restype = ctypes.c_int
-    L.accb_embedding.argtypes = [ctypes.POINTER(EmbeddingDesc), vp, vp, vp]
+    L.accb_embedding.argtypes = [vp, vp, vp, vp]
     L.accb_embedding.restype = ctypes.c_int
-    L.accb_embedding_grad.argtypes = [ctypes.POINTER(EmbeddingDesc), vp, vp, vp]
+    L.accb_embedding_grad.argtypes = [vp, vp, vp, vp]
     L.accb_embedding_grad.restype = ctypes.c_int
-    L.accb_quantize_fp8.argtypes = [ctypes.POINTER(QuantizeFp8Desc), vp, vp, vp]
+    L.accb_quantize_fp8.argtypes = [vp, vp, vp, vp]
     L.accb_quantize_fp8.restype = ctypes.c_int
-    L.accb_gemm_fp8.argtypes = [ctypes.POINTER(GemmDesc), ctypes.POINTER(Fp8Scales), vp, vp, vp, vp, vp, vp]
+    L.accb_gemm_fp8.argtypes = [vp] * 8            # descriptors as packed bytes or by reference
     L.accb_gemm_fp8.restype = ctypes.c_int
     L.accb_range_count_f32.argtypes = [ctypes.c_float, ctypes.c_float, ctypes.c_float]
     L.accb_range_count_f32.restype = ctypes.c_int64
@@ -554,29 +555,43 @@ def gather_rank2(data, indices, output, axis: int = 0) -> None:
 
 _FLOAT_KINDS = {"float32": F32, "float16": F16, "bfloat16": BF16}
 _FP8_KINDS = {"float8_e4m3fn": E4M3, "float8_e4m3": E4M3, "float8_e5m2": E5M2}
-_TORCH_CODES: dict = {}
+_FLOATS = frozenset((F32, F16, BF16))
+_FP8 = frozenset((E4M3, E5M2))
+_ONLY_F32 = frozenset((F32,))
+_IDS = frozenset((None, S32))       # None: int64
+
+# These calls take a few microseconds on the GPU at their smallest, so the path to them is kept short: descriptors are packed
+# in one go (the ctypes structures above say the same layouts field by field), and torch's attributes are read once.
+_pack_embedding = struct.Struct("@3q4i3q2f").pack
+_pack_quantize = struct.Struct("@2q4i2qq2q").pack
+_pack_gemm = struct.Struct("@3q4i6q2f2i").pack
+_pack_scales = struct.Struct("@2i4q").pack
+
+_torch_codes: dict = {}
+_torch_tensor: tuple = ()
+_raw_stream = None
 
 
-def _torch_code(name, dtype):
-    if not _TORCH_CODES:
-        import torch
-        _TORCH_CODES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3,
-                             torch.float8_e5m2: E5M2, torch.int32: S32, torch.int64: None})
-    try:
-        return _TORCH_CODES[dtype]
-    except KeyError:
-        raise TypeError(f"{name}: unsupported tensor dtype {dtype}") from None
+def _load_torch() -> None:
+    global _torch_tensor, _raw_stream
+    import torch
+    _torch_codes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3,
+                         torch.float8_e5m2: E5M2, torch.int32: S32, torch.int64: None})
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    _torch_tensor = (torch.Tensor,)
 
 
 def _operand(name: str, x, accepted, kind: Optional[str] = None):
     """-> (pointer, element type code, shape, element strides, device index or -1 for host memory) of an array whose type
     is one of `accepted` (type codes).  bf16 and 8-bit floating point numpy arrays are bit patterns (uint16, uint8) that `kind` names."""
-    if _is_torch(x):
-        code = _torch_code(name, x.dtype)
+    if isinstance(x, _torch_tensor):
+        code = _torch_codes.get(x.dtype, -1)
+        if code not in accepted:
+            raise TypeError(f"{name}: unsupported tensor dtype {x.dtype}")
         if kind is not None and code != _FLOAT_KINDS.get(kind, _FP8_KINDS.get(kind, -1)):
             raise TypeError(f"{name}: a tensor of {x.dtype} is not {kind}")
-        desc = x.data_ptr(), code, x.shape, x.stride(), (x.device.index if x.is_cuda else -1)
-    elif isinstance(x, np.ndarray):
+        return x.data_ptr(), code, x.shape, x.stride(), x.get_device()
+    if isinstance(x, np.ndarray):
         if kind == "bfloat16" and x.dtype == np.uint16:
             code = BF16
         elif kind in _FP8_KINDS and x.dtype == np.uint8:
@@ -585,72 +600,83 @@ def _operand(name: str, x, accepted, kind: Optional[str] = None):
             code = None if x.dtype == np.int64 else _NP_TYPE.get(str(x.dtype), -1)
         else:
             raise TypeError(f"{name}: an array of {x.dtype} is not {kind}")
+        if code not in accepted:
+            raise TypeError(f"{name}: unsupported element type {x.dtype}")
         if any(st % x.itemsize for st in x.strides):
             raise ValueError(f"{name}: strides must be whole elements")
-        desc = x.ctypes.data, code, x.shape, tuple(st // x.itemsize for st in x.strides), -1
+        return x.ctypes.data, code, x.shape, tuple(st // x.itemsize for st in x.strides), -1
+    if not _torch_tensor and _is_torch(x):
+        _load_torch()
+        return _operand(name, x, accepted, kind)
+    raise TypeError(f"{name}: expected a numpy array or a torch tensor")
+
+
+def _select_place(device: int) -> ctypes.CDLL:
+    """Selects a device and torch's current stream on it (-1, host arrays: the default stream) for the call that follows."""
+    L = _lib or lib()
+    if device < 0:
+        L.accb_set_stream(None)
     else:
-        raise TypeError(f"{name}: expected a numpy array or a torch tensor")
-    if code not in accepted:
-        raise TypeError(f"{name}: unsupported element type {x.dtype}")
-    return desc
+        _check(L.accb_set_device(device))
+        L.accb_set_stream(_raw_stream(device))
+    return L
 
 
-_FLOATS = (F32, F16, BF16)
-_FP8 = (E4M3, E5M2)
+def _elsewhere():
+    return ValueError("arrays must all be on one device, or all in host memory")
 
 
-def _select_for(arrays, devices) -> None:
-    """Checks that all arrays are in one place and selects its device and torch's current stream (host: the default stream)."""
-    if any(d != devices[0] for d in devices):
-        raise ValueError("arrays must all be on one device, or all in host memory")
-    _sync_torch_stream(arrays[0])
-
-
-def _positive(strides, shape):
-    """Strides of a descriptor: those of dimensions of length 0 or 1 say nothing and become at least 1."""
-    for st, n in zip(strides, shape):
-        if st < 1 and n > 1:
+def _strides2(shape, strides):
+    """The two strides of a descriptor: those of dimensions of length 0 or 1 say nothing and become at least 1."""
+    s0, s1 = strides
+    if s0 < 1 or s1 < 1:
+        if (s0 < 1 and shape[0] > 1) or (s1 < 1 and shape[1] > 1):
             raise ValueError("strides must be positive (no broadcast or reversed dimension)")
-    return [st if st > 0 else 1 for st in strides]
+        return max(s0, 1), max(s1, 1)
+    return s0, s1
 
 
-def _row_stride(name, shape, strides) -> int:
-    if shape[1] > 1 and strides[1] != 1:
+def _row_stride(name, rows, cols, s0, s1) -> int:
+    if s1 != 1 and cols > 1:
         raise ValueError(f"{name}: rows must be contiguous")
-    if shape[0] > 1 and strides[0] < shape[1]:
-        raise ValueError(f"{name}: rows must not overlap")
-    return strides[0] if shape[0] > 1 else max(1, shape[1])
+    if rows > 1:
+        if s0 < cols:
+            raise ValueError(f"{name}: rows must not overlap")
+        return s0
+    return cols or 1
 
 
-def _embedding_args(table, ids, rows, scale, beta, padding_id, table_kind, rows_kind):
+def _embedding_call(entry, table, ids, rows, scale, beta, padding_id, table_kind, rows_kind) -> None:
     pt, tt, sht, stt, dt = _operand("table", table, _FLOATS, table_kind)
-    pi, ti, shi, sti, di = _operand("ids", ids, (None, S32))
+    pi, ti, shi, sti, di = _operand("ids", ids, _IDS)
     pr, tr, shr, str_, dr = _operand("rows", rows, _FLOATS, rows_kind)
     if len(sht) != 2:
         raise ValueError("table must be rank 2")
-    if tuple(shr) != tuple(shi) + (sht[1],):
+    vocab, dim = sht
+    if shr[:-1] != shi or not shr or shr[-1] != dim:
         raise ValueError(f"shape mismatch: table{tuple(sht)} ids{tuple(shi)} rows{tuple(shr)}")
-    tokens = 1
-    expected = 1
-    for n, st in zip(reversed(shi), reversed(sti)):
-        if n > 1 and st != expected:
-            raise ValueError("ids must be contiguous")
-        expected *= n
-        tokens *= n
-    if len(shr) == 2:
-        shape2, strides2 = shr, str_
+    if len(shi) == 1 and (sti[0] == 1 or shi[0] < 2):
+        tokens, lead = shi[0], str_[0]
     else:
-        # leading dimensions must fold into one: rows a fixed distance apart
-        lead = [(n, st) for n, st in zip(shr[:-1], str_[:-1]) if n > 1]
-        for (_, outer), (n, inner) in zip(lead, lead[1:]):
+        tokens = 1
+        for n, st in zip(reversed(shi), reversed(sti)):
+            if n > 1 and st != tokens:
+                raise ValueError("ids must be contiguous")
+            tokens *= n
+        # leading dimensions of the rows must fold into one: rows a fixed distance apart
+        spaced = [(n, st) for n, st in zip(shr[:-1], str_[:-1]) if n > 1]
+        for (_, outer), (n, inner) in zip(spaced, spaced[1:]):
             if outer != n * inner:
                 raise ValueError("rows: the leading dimensions must be evenly spaced rows")
-        shape2, strides2 = (tokens, shr[-1]), (lead[-1][1] if lead else sht[1], str_[-1])
-    d = EmbeddingDesc(tokens, sht[0], sht[1], tt, tr, 8 if ti is None else 4, 0,
-                      _row_stride("table", sht, stt) if tokens else max(1, sht[1]), _row_stride("rows", shape2, strides2) if tokens else max(1, sht[1]),
-                      -1 if padding_id is None else int(padding_id), scale, beta)
-    _select_for((rows, table, ids), (dr, dt, di))
-    return d, pt, pi, pr
+        lead = spaced[-1][1] if spaced else dim
+    if dt != dr or di != dr:
+        raise _elsewhere()
+    d = _pack_embedding(tokens, vocab, dim, tt, tr, 8 if ti is None else 4, 0, _row_stride("table", vocab, dim, *stt),
+                        _row_stride("rows", tokens, dim, lead, str_[-1]), padding_id, scale, beta)
+    L = _select_place(dr)
+    rc = L.accb_embedding(d, pt, pi, pr) if entry == 0 else L.accb_embedding_grad(d, pr, pi, pt)
+    if rc < 0:
+        _check(rc)
 
 
 def embedding(table, ids, out, *, scale: float = 1.0, table_kind: Optional[str] = None, out_kind: Optional[str] = None) -> None:
@@ -661,8 +687,7 @@ def embedding(table, ids, out, *, scale: float = 1.0, table_kind: Optional[str] 
     AccbError(ERR_INDEX), for CUDA tensors from the next `synchronize()`.  `table_kind` / `out_kind` = "bfloat16" marks
     uint16 numpy arrays as bf16 bit patterns.
     """
-    d, pt, pi, po = _embedding_args(table, ids, out, scale, 0.0, None, table_kind, out_kind)
-    _check(lib().accb_embedding(ctypes.byref(d), pt, pi, po))
+    _embedding_call(0, table, ids, out, scale, 0.0, -1, table_kind, out_kind)
 
 
 def embedding_grad(grad_out, ids, grad_table, *, scale: float = 1.0, beta: float = 0.0, padding_id: Optional[int] = None,
@@ -673,10 +698,11 @@ def embedding_grad(grad_out, ids, grad_table, *, scale: float = 1.0, beta: float
     equal inputs give equal bits.  beta = 0 overwrites the whole table (words without a token become zero), beta = 1 adds to
     it - the second use of a table that is also the output layer.  Tokens with id `padding_id` add nothing.
     """
-    if padding_id is not None and padding_id < 0:
+    if padding_id is None:
+        padding_id = -1
+    elif padding_id < 0:
         raise ValueError("padding_id must not be negative (None: no padding)")
-    d, pt, pi, pr = _embedding_args(grad_table, ids, grad_out, scale, beta, padding_id, table_kind, out_kind)
-    _check(lib().accb_embedding_grad(ctypes.byref(d), pr, pi, pt))
+    _embedding_call(1, grad_table, ids, grad_out, scale, beta, padding_id, table_kind, out_kind)
 
 
 def _block_of(what: str, blocks: int, count: int) -> int:
@@ -698,17 +724,19 @@ def quantize_fp8(x, q, scales, *, kind: Optional[str] = None, q_kind: Optional[s
     """
     px, tx, shx, stx, dx = _operand("x", x, _FLOATS, kind)
     pq, tq, shq, stq, dq = _operand("q", q, _FP8, q_kind)
-    ps, _, shs, sts, ds = _operand("scales", scales, (F32,))
-    if len(shx) != 2 or tuple(shq) != tuple(shx) or len(shs) != 2:
+    ps, _, shs, sts, ds = _operand("scales", scales, _ONLY_F32)
+    if len(shx) != 2 or shq != shx or len(shs) != 2:
         raise ValueError(f"shape mismatch: x{tuple(shx)} q{tuple(shq)} scales{tuple(shs)}")
-    if shs[1] != -(-shx[1] // FP8_BLOCK):
+    rows, cols = shx
+    if shs[1] != -(-cols // FP8_BLOCK):
         raise ValueError(f"scales{tuple(shs)} must have ceil(K / {FP8_BLOCK}) columns for x{tuple(shx)}")
-    d = QuantizeFp8Desc(shx[0], shx[1], tx, tq, _block_of("scales", shs[0], shx[0]), 0)
-    d.x_stride[:] = _positive(stx, shx)
-    d.q_stride = _row_stride("q", shq, stq)
-    d.scale_stride[:] = _positive(sts, shs)
-    _select_for((x, q, scales), (dx, dq, ds))
-    _check(lib().accb_quantize_fp8(ctypes.byref(d), px, pq, ps))
+    if dq != dx or ds != dx:
+        raise _elsewhere()
+    d = _pack_quantize(rows, cols, tx, tq, _block_of("scales", shs[0], rows), 0, *_strides2(shx, stx),
+                       _row_stride("q", rows, cols, *stq), *_strides2(shs, sts))
+    rc = _select_place(dx).accb_quantize_fp8(d, px, pq, ps)
+    if rc < 0:
+        _check(rc)
 
 
 def gemm_fp8(A, B, C, a_scales, b_scales, *, bias=None, alpha: float = 1.0, beta: float = 1.0, relu: bool = False,
@@ -725,8 +753,8 @@ def gemm_fp8(A, B, C, a_scales, b_scales, *, bias=None, alpha: float = 1.0, beta
     pa, ta, sha, sta, da = _operand("A", A, _FP8, a_kind)
     pb, tb, shb, stb, db = _operand("B", B, _FP8, b_kind)
     pc, tc, shc, stc, dc = _operand("C", C, _FLOATS, out_kind)
-    psa, _, shsa, stsa, dsa = _operand("a_scales", a_scales, (F32,))
-    psb, _, shsb, stsb, dsb = _operand("b_scales", b_scales, (F32,))
+    psa, _, shsa, stsa, dsa = _operand("a_scales", a_scales, _ONLY_F32)
+    psb, _, shsb, stsb, dsb = _operand("b_scales", b_scales, _ONLY_F32)
     if not len(sha) == len(shb) == len(shc) == len(shsa) == len(shsb) == 2:
         raise ValueError("gemm_fp8 operands and scales must be rank 2")
     m, k = sha
@@ -736,23 +764,21 @@ def gemm_fp8(A, B, C, a_scales, b_scales, *, bias=None, alpha: float = 1.0, beta
     blocks = -(-k // FP8_BLOCK)
     if shsa[1] != blocks or shsb[0] != blocks:
         raise ValueError(f"scales of A{tuple(shsa)} and B{tuple(shsb)} must cover {blocks} blocks of K")
-    devices = [dc, da, db, dsa, dsb]
+    if da != dc or db != dc or dsa != dc or dsb != dc:
+        raise _elsewhere()
     pbias = None
     if bias is not None:
-        pbias, _, shbias, stbias, dbias = _operand("bias", bias, (F32,))
-        if tuple(shbias) != (n,) or (n > 1 and stbias[0] != 1):
+        pbias, _, shbias, stbias, dbias = _operand("bias", bias, _ONLY_F32)
+        if len(shbias) != 1 or shbias[0] != n or (n > 1 and stbias[0] != 1):
             raise ValueError("bias must be contiguous fp32 of length N")
-        devices.append(dbias)
-    d = GemmDesc(m, n, k, ta, tb, tc, _COMPUTE[compute])
-    d.a_stride[:] = _positive(sta, sha)
-    d.b_stride[:] = _positive(stb, shb)
-    d.c_stride[:] = _positive(stc, shc)
-    d.alpha, d.beta, d.epilogue, d.max_ctas = alpha, beta, EPI_RELU if relu else EPI_NONE, max_ctas
-    s = Fp8Scales(_block_of("a_scales", shsa[0], m), _block_of("b_scales", shsb[1], n))
-    s.a_stride[:] = _positive(stsa, shsa)
-    s.b_stride[:] = _positive(stsb, shsb)
-    _select_for((C,), devices)
-    _check(lib().accb_gemm_fp8(ctypes.byref(d), ctypes.byref(s), pa, pb, pc, psa, psb, pbias))
+        if dbias != dc:
+            raise _elsewhere()
+    d = _pack_gemm(m, n, k, ta, tb, tc, _COMPUTE[compute], *_strides2(sha, sta), *_strides2(shb, stb), *_strides2(shc, stc),
+                   alpha, beta, EPI_RELU if relu else EPI_NONE, max_ctas)
+    s = _pack_scales(_block_of("a_scales", shsa[0], m), _block_of("b_scales", shsb[1], n), *_strides2(shsa, stsa), *_strides2(shsb, stsb))
+    rc = _select_place(dc).accb_gemm_fp8(d, s, pa, pb, pc, psa, psb, pbias)
+    if rc < 0:
+        _check(rc)
 
 
 def range_count(start, limit, delta) -> int:

@@ -38,6 +38,19 @@ def test_embedding_arguments():
         rt.embedding(t, ids, out, table_kind="bfloat16")
 
 
+def test_packed_descriptors_have_the_structures_layout():
+    for pack, kind, values in [(rt._pack_embedding, rt.EmbeddingDesc, (1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11.0, 12.0)),
+                               (rt._pack_quantize, rt.QuantizeFp8Desc, (1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11)),
+                               (rt._pack_gemm, rt.GemmDesc, (1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14.0, 15.0, 16, 17)),
+                               (rt._pack_scales, rt.Fp8Scales, (1, 2, 3, 4, 5, 6))]:
+        d = kind.from_buffer_copy(pack(*values))
+        flat = []
+        for name, _ in kind._fields_:
+            v = getattr(d, name)
+            flat += list(v) if isinstance(v, ctypes.Array) else [v]
+        assert tuple(flat) == values and len(pack(*values)) == ctypes.sizeof(kind)
+
+
 def test_embedding_descriptor():
     p = ctypes.c_void_p(64)
     good = dict(tokens=3, vocab=9, dim=8, table_type=rt.F32, rows_type=rt.BF16, id_bytes=8, reserved=0, table_stride=8, rows_stride=8, padding_id=-1, scale=1.0, beta=0.0)
