@@ -18,6 +18,19 @@ namespace {
 
 template <typename T, int E> struct alignas(E * sizeof(T) > 16 ? 16 : E * sizeof(T)) Vec { T v[E]; };
 
+// a store that should not displace what is read again (the table) from L2
+template <typename T, int E>
+__device__ __forceinline__ void store_streaming(T* dst, const Vec<T, E>& x)
+{
+    constexpr int kBytes = E * (int)sizeof(T);
+    if constexpr (kBytes % 16 == 0) {
+        const uint4* w = reinterpret_cast<const uint4*>(&x);
+#pragma unroll
+        for (int i = 0; i < kBytes / 16; ++i) __stcs(reinterpret_cast<uint4*>(dst) + i, w[i]);
+    } else if constexpr (kBytes == 8) __stcs(reinterpret_cast<uint2*>(dst), *reinterpret_cast<const uint2*>(&x));
+    else *reinterpret_cast<Vec<T, E>*>(dst) = x;
+}
+
 // ---------------------------------------------------------------------------------
 // lookup
 // ---------------------------------------------------------------------------------
@@ -72,7 +85,7 @@ embedding_kernel(const TT* __restrict__ table, const void* __restrict__ ids, TR*
         Vec<TR, E> y;
 #pragma unroll
         for (int e = 0; e < E; ++e) y.v[e] = ok[u] ? (TR)((float)x[u].v[e] * p.scale) : (TR)0.0f;
-        *reinterpret_cast<Vec<TR, E>*>(rows + (int64_t)row[u] * p.rows_stride + (int64_t)col[u] * E) = y;
+        store_streaming<TR, E>(rows + (int64_t)row[u] * p.rows_stride + (int64_t)col[u] * E, y);
     }
 }
 
@@ -233,11 +246,63 @@ __device__ void sort_tokens(const void* ids, int* keys0, int* tokens0, int* keys
     if (lane == 0 && bad) { atomicAdd(status + ST_EMBED_COUNT, bad); status[ST_EMBED_ID] = p.launch_id; }
 }
 
+// What step 1 does beside sorting: words without a token get their final value, zero or beta times the old one.  That is
+// writing most of the table, which HBM bounds, while the sort is bound by latency: clusters 1 .. of the launch do it
+// while cluster 0 sorts.  A CTA owns a run of rows and learns from all ids, in shared memory, which of them have tokens.
+struct ClearParams {
+    int64_t stride;
+    int dim;
+    int vec;                     // rows are whole 16-byte vectors, 16-byte aligned
+    float beta;
+    int rows_per_cta;
+};
+
+// seen: (rows_per_cta + 31) / 32 words of shared memory
+template <typename TT, int kThreads>
+__device__ __forceinline__ void clear_rows(TT* table, const void* ids, int part, const SortParams& p, const ClearParams& c, uint32_t* seen)
+{
+    const int64_t first = (int64_t)part * c.rows_per_cta;
+    const int rows = (int)(p.vocab - first < c.rows_per_cta ? p.vocab - first : c.rows_per_cta);
+    if (rows <= 0) return;
+    for (int i = threadIdx.x; i < (rows + 31) / 32; i += kThreads) seen[i] = 0u;
+    __syncthreads();
+#pragma unroll 8
+    for (int i = threadIdx.x; i < p.n; i += kThreads) {
+        const int64_t id = load_id(ids, i, p.id_bytes), at = id - first;
+        if ((uint64_t)at < (uint64_t)rows && id != p.padding_id) atomicOr(seen + at / 32, 1u << (at % 32));
+    }
+    __syncthreads();
+    constexpr int V = 16 / (int)sizeof(TT);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    for (int r = warp; r < rows; r += kThreads / 32) {
+        if (seen[r / 32] >> (r % 32) & 1u) continue;
+        TT* row = table + (first + r) * c.stride;
+        if (c.beta == 0.0f) {
+            if (c.vec) {
+#pragma unroll 8
+                for (int v = lane; v < c.dim / V; v += 32) __stcs(reinterpret_cast<uint4*>(row) + v, make_uint4(0u, 0u, 0u, 0u));
+            } else {
+                for (int i = lane; i < c.dim; i += 32) row[i] = (TT)0.0f;
+            }
+        } else {
+            for (int i = lane; i < c.dim; i += 32) row[i] = (TT)(c.beta * (float)row[i]);
+        }
+    }
+}
+
+template <typename TT>
 __global__ void __launch_bounds__(kSortThreads, 1)
-sort_tokens_kernel(const void* __restrict__ ids, int* keys0, int* tokens0, int* keys1, int* tokens1, int* status, const SortParams p)
+sort_tokens_kernel(const void* __restrict__ ids, int* keys0, int* tokens0, int* keys1, int* tokens1, int* long_words, TT* __restrict__ table, int* status,
+                   const SortParams p, const ClearParams c)
 {
     extern __shared__ int smem[];
     pdl_enter();
+    const int ctas = (int)cluster_size();
+    if ((int)blockIdx.x >= ctas) {
+        clear_rows<TT, kSortThreads>(table, ids, (int)blockIdx.x - ctas, p, c, reinterpret_cast<uint32_t*>(smem));
+        return;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) *long_words = 0;
     sort_tokens(ids, keys0, tokens0, keys1, tokens1, status, p, smem);
 }
 
@@ -281,7 +346,7 @@ __device__ __forceinline__ void write_sum(TT* table, int64_t word, int64_t strid
 template <typename TT, typename TR, int E>
 __global__ void __launch_bounds__(kSumThreads)
 sum_rows_kernel(const TR* __restrict__ rows, const int* __restrict__ keys, const int* __restrict__ tokens, TT* __restrict__ table,
-                float* __restrict__ partial, int* __restrict__ runs_on, const SumParams p)
+                float* __restrict__ partial, int* __restrict__ long_words, const SumParams p)
 {
     pdl_enter();
     const int chunk = blockIdx.x / p.slabs, slab = blockIdx.x % p.slabs;
@@ -295,31 +360,36 @@ sum_rows_kernel(const TR* __restrict__ rows, const int* __restrict__ keys, const
     __syncthreads();
     const int* k = key + kChunk;                             // k[i] = key of place i0 + i
     const int len = i1 - i0;
+    // Lane l of every warp looks at places l - kChunk, l and l + kChunk of the chunk; ballots give the runs of equal keys.
+    static_assert(kChunk == 32, "one place a lane");
+    const int lane = threadIdx.x % 32;
+    const int k_first = k[0], k_last = k[len - 1];
+    const uint32_t before = __ballot_sync(0xffffffffu, k[lane - kChunk] == k_first);
+    const uint32_t same_first = __ballot_sync(0xffffffffu, k[lane] == k_first), beyond_first = __ballot_sync(0xffffffffu, k[lane + kChunk] == k_first);
+    const uint32_t same_last = __ballot_sync(0xffffffffu, k[lane] == k_last), beyond_last = __ballot_sync(0xffffffffu, k[lane + kChunk] == k_last);
+    auto ones = [](uint32_t m) { return m == 0xffffffffu ? 32 : __ffs(~m) - 1; };            // consecutive ones from bit 0
+    const int back = before == 0xffffffffu ? 32 : __clz(~before);
+    const int ahead_first = same_first == 0xffffffffu ? 32 + ones(beyond_first) : ones(same_first);
     // the piece of a word that began earlier: skipped when that word is short (its first chunk takes it all)
     int first = 0;
     bool first_long = false;
-    if (k[-1] == k[0]) {
-        int back = 1, ahead = 0;
-        while (back < kChunk && k[-back - 1] == k[0]) ++back;
-        while (ahead < 2 * kChunk && k[ahead] == k[0]) ++ahead;
-        first_long = back + ahead > kChunk;
-        if (!first_long) first = ahead < len ? ahead : len;
+    if (back > 0) {
+        first_long = back + ahead_first > kChunk;
+        if (!first_long) first = ahead_first < len ? ahead_first : len;
     }
     // the word that runs past the chunk's end: taken to its end when short, to the border when long
     int last = len;
     bool last_long = false;
-    if (first < len && i1 < p.n && k[len] == k[len - 1]) {
-        const int w = k[len - 1];
-        int start = len - 1, ahead = len;
-        while (start > 0 && k[start - 1] == w) --start;
-        const bool from_before = start == 0 && k[-1] == w;
-        while (ahead < 2 * kChunk && k[ahead] == w) ++ahead;
-        if (!from_before) {
-            last_long = ahead - start > kChunk;
-            if (!last_long) last = ahead;
+    if (first < len && len == kChunk && (beyond_last & 1u)) {
+        const uint32_t other = ~same_last;                                                    // the list is sorted
+        const int start = other ? 32 - __clz(other) : 0;
+        const int end = kChunk + ones(beyond_last);
+        if (start > 0 || back == 0) {
+            last_long = end - start > kChunk;
+            if (!last_long) last = end;
         }
     }
-    if (threadIdx.x == 0 && slab == 0) runs_on[chunk] = last_long;
+    if (threadIdx.x == 0 && slab == 0 && last_long && k_last < p.vocab) long_words[1 + atomicAdd(long_words, 1)] = chunk;
     const int col = (slab * kSumThreads + threadIdx.x) * E;
     if (col >= p.dim) return;
     float acc[E] = {};
@@ -353,37 +423,44 @@ sum_rows_kernel(const TR* __restrict__ rows, const int* __restrict__ keys, const
     }
 }
 
-// step 3: the pieces of the long words.  Lane l of a warp looks at chunk 32 * blockIdx.x + l; the block then takes the long
-// words that begin there one by one: kJoinLanes threads a column add every kJoinLanes-th piece, and their sums are added
-// in lane order.
-constexpr int kJoinCols = 32, kJoinLanes = 8;
+// step 3: the pieces of the long words.  long_words[0] of them begin in chunks long_words[1 ..] (in any order: each is a sum
+// of its own).  A block takes kJoinCols columns of one word at a time: kJoinLanes threads a column add every kJoinLanes-th
+// piece, and their sums are added in lane order.
+constexpr int kJoinCols = 32, kJoinLanes = 16;
 
 template <typename TT>
 __global__ void __launch_bounds__(kJoinCols * kJoinLanes)
-join_rows_kernel(const float* __restrict__ partial, const int* __restrict__ keys, const int* __restrict__ runs_on, TT* __restrict__ table,
+join_rows_kernel(const float* __restrict__ partial, const int* __restrict__ keys, const int* __restrict__ long_words, TT* __restrict__ table,
                  const SumParams p)
 {
     pdl_enter();
     __shared__ float part[kJoinLanes][kJoinCols];
     const int x = threadIdx.x % kJoinCols, y = threadIdx.x / kJoinCols;
-    const int base = blockIdx.x * 32;
-    uint32_t todo = __ballot_sync(0xffffffffu, base + x < p.chunks && runs_on[base + x]);
-    const int col = blockIdx.y * kJoinCols + x;
-    while (todo) {
-        const int chunk = base + __ffs(todo) - 1;
-        todo &= todo - 1;
+    const int col_blocks = (p.dim + kJoinCols - 1) / kJoinCols;
+    const int64_t total = (int64_t)long_words[0] * col_blocks;
+    for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
+        const int chunk = long_words[1 + w / col_blocks], col = (int)(w % col_blocks) * kJoinCols + x;
         const int word = keys[chunk * kChunk + kChunk - 1];
-        // the word's last place: the list is sorted
+        // the first place behind the word, found by each warp for itself with 32 probes a step of the sorted list
         int lo = chunk * kChunk + kChunk, hi = p.n;
-        while (lo < hi) { const int mid = lo + (hi - lo) / 2; if (keys[mid] <= word) lo = mid + 1; else hi = mid; }
+        while (lo < hi) {
+            const int step = (hi - lo + 31) / 32;
+            const int64_t at = lo + (int64_t)x * step;
+            const int inside = __popc(__ballot_sync(0xffffffffu, at < hi && keys[at] <= word));
+            // probe `inside` lies behind the word (or the range), the one before it does not
+            if (inside < 32) hi = (int)min((int64_t)hi, lo + (int64_t)inside * step);
+            if (inside > 0) lo += (inside - 1) * step + 1;
+        }
         const int last_chunk = (lo - 1) / kChunk;
         float acc = 0.0f;
-        if (col < p.dim && word < p.vocab)
+        if (col < p.dim) {
+#pragma unroll 4
             for (int c = chunk + y; c <= last_chunk; c += kJoinLanes)
-                acc += partial[((int64_t)c * 2 + (c == chunk ? 1 : 0)) * p.dim + col];
+                acc += __ldcs(partial + ((int64_t)c * 2 + (c == chunk ? 1 : 0)) * p.dim + col);
+        }
         part[y][x] = acc;
         __syncthreads();
-        if (y == 0 && col < p.dim && word < p.vocab) {
+        if (y == 0 && col < p.dim) {
             float sum[1] = { 0.0f };
 #pragma unroll
             for (int l = 0; l < kJoinLanes; ++l) sum[0] += part[l][x];
@@ -393,59 +470,212 @@ join_rows_kernel(const float* __restrict__ partial, const int* __restrict__ keys
     }
 }
 
-// Rows of the table before any sum is added: zero (beta = 0) or scaled by beta.  `touched` words are overwritten afterwards
-// when beta = 0; with another beta the sums read the old value themselves, so only untouched words are scaled here.
-template <typename TT>
-__global__ void __launch_bounds__(256)
-untouched_rows_kernel(const int* __restrict__ keys, int n, TT* __restrict__ table, int64_t vocab, int64_t dim, int64_t stride, float beta)
+// ---------------------------------------------------------------------------------
+// gradient of few tokens: one launch, no workspace
+// ---------------------------------------------------------------------------------
+// Up to kFewTokens tokens, every block can look at all of them.  The block of (token, slab of columns) does nothing unless
+// it is its word's first token; else it collects the word's tokens in order and adds their rows: a thread one vector of
+// columns, or, for more than kFewSplit tokens, kFewLanes threads a vector, each a kFewLanes-th of the list, whose
+// sums are added in lane order.  Blocks behind those give words without a token their value.
+constexpr int kFewTokens = 1024, kFewThreads = 256, kFewLanes = 8, kFewSplit = 16, kFewUnroll = 8;
+
+template <typename TT, typename TR, int E>
+__global__ void __launch_bounds__(kFewThreads)
+few_tokens_kernel(const TR* __restrict__ rows, const void* __restrict__ ids, TT* __restrict__ table, int* __restrict__ status, const SortParams sp,
+                  const ClearParams c, const SumParams p)
 {
     pdl_enter();
-    for (int64_t v = blockIdx.x; v < vocab; v += gridDim.x) {
-        int lo = 0, hi = n;
-        while (lo < hi) { const int mid = lo + (hi - lo) / 2; if (keys[mid] < v) lo = mid + 1; else hi = mid; }
-        if (lo < n && keys[lo] == v) continue;
-        TT* row = table + v * stride;
-        if (beta == 0.0f) for (int64_t c = threadIdx.x; c < dim; c += 256) row[c] = (TT)0.0f;
-        else for (int64_t c = threadIdx.x; c < dim; c += 256) row[c] = (TT)(beta * (float)row[c]);
+    constexpr int kWarps = kFewThreads / 32, kRounds = kFewTokens / kFewThreads;
+    __shared__ uint32_t list[kFewTokens];
+    __shared__ int count[kRounds][kWarps];
+    __shared__ float part[kFewLanes][kFewThreads / kFewLanes][E + 1];
+    const int sum_blocks = sp.n * p.slabs;
+    if ((int)blockIdx.x >= sum_blocks) {
+        clear_rows<TT, kFewThreads>(table, ids, (int)blockIdx.x - sum_blocks, sp, c, list);
+        return;
+    }
+    const int token = blockIdx.x / p.slabs, slab = blockIdx.x % p.slabs;
+    const int64_t word = load_id(ids, token, sp.id_bytes);
+    const bool good = (uint64_t)word < (uint64_t)sp.vocab;
+    if (!good || word == sp.padding_id) {
+        if (!good && word != sp.padding_id && slab == 0 && threadIdx.x == 0) { atomicAdd(status + ST_EMBED_COUNT, 1); status[ST_EMBED_ID] = sp.launch_id; }
+        return;
+    }
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    uint32_t mine[kRounds];
+    bool earlier = false;
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+        const int i = r * kFewThreads + threadIdx.x;
+        const bool same = i < sp.n && load_id(ids, i, sp.id_bytes) == word;
+        earlier |= same && i < token;
+        mine[r] = __ballot_sync(0xffffffffu, same);
+        if (lane == 0) count[r][warp] = __popc(mine[r]);
+    }
+    if (__syncthreads_or(earlier)) return;
+    int n = 0;
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r)
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w == warp && (mine[r] >> lane & 1u)) list[n + __popc(mine[r] & ((1u << lane) - 1u))] = (uint32_t)(r * kFewThreads + threadIdx.x);
+            n += count[r][w];
+        }
+    __syncthreads();
+    auto add_rows = [&](int begin, int step, int col, float (&acc)[E]) {
+        for (int j0 = begin; j0 < n; j0 += step * kFewUnroll) {
+            Vec<TR, E> x[kFewUnroll];
+#pragma unroll
+            for (int u = 0; u < kFewUnroll; ++u)
+                if (j0 + u * step < n) x[u] = *reinterpret_cast<const Vec<TR, E>*>(rows + (int64_t)list[j0 + u * step] * p.rows_stride + col);
+#pragma unroll
+            for (int u = 0; u < kFewUnroll; ++u)
+                if (j0 + u * step < n) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] += (float)x[u].v[e];
+                }
+        }
+    };
+    if (n <= kFewSplit) {
+        const int col = (slab * kFewThreads + threadIdx.x) * E;
+        if (col >= p.dim) return;
+        float acc[E] = {};
+        add_rows(0, 1, col, acc);
+        write_sum<TT, E>(table, word, p.table_stride, col, acc, p.scale, p.beta);
+        return;
+    }
+    constexpr int kCols = kFewThreads / kFewLanes;
+    const int x = threadIdx.x % kCols, y = threadIdx.x / kCols;
+    for (int v0 = 0; v0 < kFewThreads; v0 += kCols) {
+        const int col = (slab * kFewThreads + v0 + x) * E;
+        float acc[E] = {};
+        if (col < p.dim) add_rows(y, kFewLanes, col, acc);
+#pragma unroll
+        for (int e = 0; e < E; ++e) part[y][x][e] = acc[e];
+        __syncthreads();
+        if (y == 0 && col < p.dim) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                acc[e] = 0.0f;
+#pragma unroll
+                for (int l = 0; l < kFewLanes; ++l) acc[e] += part[l][x][e];
+            }
+            write_sum<TT, E>(table, word, p.table_stride, col, acc, p.scale, p.beta);
+        }
+        __syncthreads();
     }
 }
 
-struct GradWork { int *keys0, *tokens0, *keys1, *tokens1, *runs_on; float* partial; };
+// Vectors of a row for the gradient kernels: 16 bytes of the rows that are read, however many that are of the table
+template <typename TT, typename TR>
+bool vector_rows(const accb_embedding_desc& d, const void* table, const void* rows)
+{
+    constexpr int E = 16 / (int)sizeof(TR);
+    constexpr size_t kTableAlign = E * sizeof(TT) > 16 ? 16 : E * sizeof(TT);
+    return d.dim % E == 0 && d.rows_stride % E == 0 && (d.table_stride * sizeof(TT)) % kTableAlign == 0 && (reinterpret_cast<uintptr_t>(rows) & 15) == 0 &&
+           reinterpret_cast<uintptr_t>(table) % kTableAlign == 0;
+}
+
+template <typename TT>
+ClearParams clear_params(const accb_embedding_desc& d, const void* table, int64_t ctas)
+{
+    ClearParams c;
+    c.stride = d.table_stride; c.dim = (int)d.dim; c.beta = d.beta;
+    c.vec = (d.dim * sizeof(TT)) % 16 == 0 && (d.table_stride * sizeof(TT)) % 16 == 0 && (reinterpret_cast<uintptr_t>(table) & 15) == 0;
+    c.rows_per_cta = (int)((d.vocab + ctas - 1) / ctas);
+    return c;
+}
 
 template <typename TT, typename TR>
-cudaError_t launch_sums(const EmbeddingLaunch& l, const void* rows, void* table, const GradWork& w, const int* keys, const int* tokens)
+int launch_grad(const EmbeddingLaunch& l, const void* rows, void* table, const char** err)
 {
     const accb_embedding_desc& d = l.d;
-    constexpr int E = 16 / (int)(sizeof(TT) > sizeof(TR) ? sizeof(TT) : sizeof(TR));
-    auto aligned = [](const void* p, int64_t stride, int64_t es) { return (reinterpret_cast<uintptr_t>(p) % (E * es)) == 0 && stride % E == 0; };
-    const bool vec = d.dim % E == 0 && aligned(table, d.table_stride, sizeof(TT)) && aligned(rows, d.rows_stride, sizeof(TR));
-    cudaError_t e = cudaSuccess;
-    if (d.beta != 1.0f) {
-        const unsigned blocks = (unsigned)(d.vocab < 148 * 16 ? d.vocab : 148 * 16);
-        e = launch_pdl(untouched_rows_kernel<TT>, dim3(blocks), dim3(256), l.stream, keys, (int)d.tokens, (TT*)table, d.vocab, d.dim, d.table_stride, d.beta);
-        if (e != cudaSuccess) return e;
-    }
-    if (d.tokens == 0) return cudaSuccess;
+    constexpr int E = 16 / (int)sizeof(TR);
+    const int64_t n = d.tokens;
+    const bool vec = vector_rows<TT, TR>(d, table, rows), clear = d.beta != 1.0f;
+    SortParams s;
+    s.n = (int)n; s.vocab = (int)d.vocab; s.padding_id = d.padding_id < 0 ? INT64_MIN : d.padding_id;   // (an id of -1 is out of range, not padding)
+    s.id_bytes = d.id_bytes;
+    int bits = 1;
+    while (((int64_t)1 << bits) <= d.vocab) ++bits;          // keys 0 .. vocab
+    s.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
+    s.digit_bits = (bits + s.passes - 1) / s.passes;
+    s.launch_id = l.launch_id;
     SumParams p;
-    p.n = (int)d.tokens; p.vocab = (int)d.vocab; p.dim = (int)d.dim;
+    p.n = (int)n; p.vocab = (int)d.vocab; p.dim = (int)d.dim;
     p.table_stride = d.table_stride; p.rows_stride = d.rows_stride;
     p.scale = d.scale; p.beta = d.beta;
-    p.chunks = (p.n + kChunk - 1) / kChunk;
+    p.chunks = (int)((n + kChunk - 1) / kChunk);
+    static_assert(kSumThreads == kFewThreads, "one slab width");
     const int64_t cols_per_slab = (int64_t)kSumThreads * (vec ? E : 1);
     p.slabs = (int)((d.dim + cols_per_slab - 1) / cols_per_slab);
-    if ((int64_t)p.chunks * p.slabs > 0x7fffffff || (d.dim + kJoinCols - 1) / kJoinCols > 65535) return cudaErrorInvalidConfiguration;
-    const dim3 grid((unsigned)(p.chunks * p.slabs)), block(kSumThreads);
-    e = vec ? launch_pdl(sum_rows_kernel<TT, TR, E>, grid, block, l.stream, (const TR*)rows, keys, tokens, (TT*)table, w.partial, w.runs_on, p)
-            : launch_pdl(sum_rows_kernel<TT, TR, 1>, grid, block, l.stream, (const TR*)rows, keys, tokens, (TT*)table, w.partial, w.runs_on, p);
-    if (e != cudaSuccess) return e;
-    return launch_pdl(join_rows_kernel<TT>, dim3((unsigned)((p.chunks + 31) / 32), (unsigned)((d.dim + kJoinCols - 1) / kJoinCols)),
-                      dim3(kJoinCols * kJoinLanes), l.stream, (const float*)w.partial, keys, (const int*)w.runs_on, (TT*)table, p);
+    auto cuda_failed = [&](cudaError_t e) { *err = cudaGetErrorString(e); return (int)ACCB_ERR_CUDA; };
+
+    if (n <= kFewTokens) {
+        // a few rows a clearing block, four blocks an SM, and no more rows than a block's bit list holds
+        const int64_t most = (int64_t)kFewTokens * 32;
+        int64_t ctas = clear ? (d.vocab + 7) / 8 : 0;
+        if (ctas > 4 * l.num_sms) ctas = 4 * l.num_sms;
+        if (clear && (d.vocab + most - 1) / most > ctas) ctas = (d.vocab + most - 1) / most;
+        const ClearParams c = clear_params<TT>(d, table, ctas > 0 ? ctas : 1);
+        const dim3 grid((unsigned)(n * p.slabs + ctas)), block(kFewThreads);
+        const cudaError_t e = vec ? launch_pdl(few_tokens_kernel<TT, TR, E>, grid, block, l.stream, (const TR*)rows, l.ids, (TT*)table, l.status, s, c, p)
+                                  : launch_pdl(few_tokens_kernel<TT, TR, 1>, grid, block, l.stream, (const TR*)rows, l.ids, (TT*)table, l.status, s, c, p);
+        if (e != cudaSuccess) return cuda_failed(e);
+        note_launches(1);
+        return 1;
+    }
+
+    const int64_t blocks = (int64_t)p.chunks * p.slabs;
+    if (blocks > 0x7fffffff) return cuda_failed(cudaErrorInvalidConfiguration);
+    const size_t list = ((size_t)n * 4 + 15) / 16 * 16, words = ((size_t)(p.chunks + 1) * 4 + 15) / 16 * 16;
+    char* ws = (char*)temp_alloc(l.device, 4 * list + words + (size_t)p.chunks * 2 * (size_t)d.dim * 4, l.stream);
+    if (!ws) { *err = "no device memory for the workspace"; return ACCB_ERR_CUDA; }
+    int *keys0 = (int*)ws, *tokens0 = (int*)(ws + list), *keys1 = (int*)(ws + 2 * list), *tokens1 = (int*)(ws + 3 * list), *long_words = (int*)(ws + 4 * list);
+    float* partial = (float*)(ws + 4 * list + words);
+    const int* keys = (s.passes & 1) ? keys0 : keys1;
+    const int* tokens = (s.passes & 1) ? tokens0 : tokens1;
+    cudaError_t e = cudaSuccess;
+    {
+        auto kernel = sort_tokens_kernel<TT>;
+        static std::atomic<bool> opted[64];
+        if (l.device >= 64 || !opted[l.device].load(std::memory_order_acquire)) {
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSortSmem);
+            if (e == cudaSuccess && l.device < 64) opted[l.device].store(true, std::memory_order_release);
+        }
+        const int cluster = n <= 2048 ? 1 : n <= 4096 ? 2 : n <= 8192 ? 4 : kSortCluster;
+        // one clearing CTA an SM beside the sorting cluster; more only where a CTA's bit list (its shared memory) ends
+        const int64_t most = (int64_t)(kSortSmem / 4) * 32, need = (d.vocab + most - 1) / most;
+        int64_t ctas = clear ? (l.num_sms - cluster) / cluster * cluster : 0;
+        if (clear && need > ctas) ctas = (need + cluster - 1) / cluster * cluster;
+        const ClearParams c = clear_params<TT>(d, table, ctas > 0 ? ctas : 1);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(cluster + ctas)); cfg.blockDim = dim3(kSortThreads); cfg.dynamicSmemBytes = kSortSmem; cfg.stream = l.stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = options().stream_pdl == 0 ? 0 : 1;
+        cfg.attrs = attr; cfg.numAttrs = 2;
+        if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, l.ids, keys0, tokens0, keys1, tokens1, long_words, (TT*)table, l.status, s, c);
+    }
+    const dim3 grid((unsigned)blocks), block(kSumThreads);
+    if (e == cudaSuccess)
+        e = vec ? launch_pdl(sum_rows_kernel<TT, TR, E>, grid, block, l.stream, (const TR*)rows, keys, tokens, (TT*)table, partial, long_words, p)
+                : launch_pdl(sum_rows_kernel<TT, TR, 1>, grid, block, l.stream, (const TR*)rows, keys, tokens, (TT*)table, partial, long_words, p);
+    if (e == cudaSuccess)
+        e = launch_pdl(join_rows_kernel<TT>, dim3((unsigned)(4 * l.num_sms)), dim3(kJoinCols * kJoinLanes), l.stream, (const float*)partial, keys,
+                       (const int*)long_words, (TT*)table, p);
+    temp_free(ws, l.stream);
+    if (e != cudaSuccess) return cuda_failed(e);
+    note_launches(3);
+    return 3;
 }
 
 template <template <typename, typename> class F, typename... Args>
-cudaError_t by_types(int table_type, int rows_type, Args... args)
+auto by_types(int table_type, int rows_type, Args... args)
 {
-    auto rows = [&](auto tt) -> cudaError_t {
+    auto rows = [&](auto tt) {
         using TT = decltype(tt);
         if (rows_type == ACCB_F32) return F<TT, float>::run(args...);
         if (rows_type == ACCB_F16) return F<TT, __half>::run(args...);
@@ -458,11 +688,8 @@ cudaError_t by_types(int table_type, int rows_type, Args... args)
 template <typename TT, typename TR> struct Lookup {
     static cudaError_t run(const EmbeddingLaunch* l, const void* table, void* rows) { return launch_lookup<TT, TR>(*l, table, rows); }
 };
-template <typename TT, typename TR> struct Sums {
-    static cudaError_t run(const EmbeddingLaunch* l, const void* rows, void* table, const GradWork* w, const int* keys, const int* tokens)
-    {
-        return launch_sums<TT, TR>(*l, rows, table, *w, keys, tokens);
-    }
+template <typename TT, typename TR> struct Grad {
+    static int run(const EmbeddingLaunch* l, const void* rows, void* table, const char** err) { return launch_grad<TT, TR>(*l, rows, table, err); }
 };
 
 }  // namespace
@@ -477,51 +704,8 @@ int launch_embedding(const EmbeddingLaunch& l, const void* table, void* rows, co
 
 int launch_embedding_grad(const EmbeddingLaunch& l, const void* rows, void* table, const char** err)
 {
-    const accb_embedding_desc& d = l.d;
-    const int64_t n = d.tokens;
-    if (n == 0 && d.beta == 1.0f) return 0;
-    const int64_t chunks = (n + kChunk - 1) / kChunk;
-    const size_t list = ((size_t)n * 4 + 15) / 16 * 16;
-    const size_t bytes = 4 * list + ((size_t)chunks * 4 + 15) / 16 * 16 + (size_t)chunks * 2 * (size_t)d.dim * 4 + 16;
-    char* ws = (char*)temp_alloc(l.device, bytes, l.stream);
-    if (!ws) { *err = "no device memory for the workspace"; return ACCB_ERR_CUDA; }
-    GradWork w;
-    w.keys0 = (int*)ws; w.tokens0 = (int*)(ws + list); w.keys1 = (int*)(ws + 2 * list); w.tokens1 = (int*)(ws + 3 * list);
-    w.runs_on = (int*)(ws + 4 * list);
-    w.partial = (float*)(ws + 4 * list + ((size_t)chunks * 4 + 15) / 16 * 16);
-
-    SortParams s;
-    s.n = (int)n; s.vocab = (int)d.vocab; s.padding_id = d.padding_id < 0 ? -1 : d.padding_id; s.id_bytes = d.id_bytes;
-    int bits = 1;
-    while (((int64_t)1 << bits) <= d.vocab) ++bits;          // keys 0 .. vocab
-    s.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
-    s.digit_bits = (bits + s.passes - 1) / s.passes;
-    s.launch_id = l.launch_id;
-    const int* keys = (s.passes & 1) ? w.keys0 : w.keys1;
-    const int* tokens = (s.passes & 1) ? w.tokens0 : w.tokens1;
-    cudaError_t e = cudaSuccess;
-    if (n > 0) {
-        static std::atomic<bool> opted[64];
-        if (l.device < 0 || l.device >= 64 || !opted[l.device]) {
-            e = cudaFuncSetAttribute(sort_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSortSmem);
-            if (e == cudaSuccess && l.device >= 0 && l.device < 64) opted[l.device] = true;
-        }
-        const unsigned ctas = n <= 2048 ? 1 : n <= 4096 ? 2 : n <= 8192 ? 4 : kSortCluster;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(kSortThreads); cfg.dynamicSmemBytes = kSortSmem; cfg.stream = l.stream;
-        cudaLaunchAttribute attr[2];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[1].val.programmaticStreamSerializationAllowed = options().stream_pdl == 0 ? 0 : 1;
-        cfg.attrs = attr; cfg.numAttrs = 2;
-        if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, sort_tokens_kernel, l.ids, w.keys0, w.tokens0, w.keys1, w.tokens1, l.status, s);
-    }
-    if (e == cudaSuccess) e = by_types<Sums>(d.table_type, d.rows_type, &l, rows, table, (const GradWork*)&w, keys, tokens);
-    temp_free(ws, l.stream);
-    if (e != cudaSuccess) { *err = cudaGetErrorString(e); return ACCB_ERR_CUDA; }
-    note_launches((n > 0 ? 3 : 0) + (d.beta != 1.0f ? 1 : 0));
-    return 1;
+    if (l.d.tokens == 0 && l.d.beta == 1.0f) return 0;
+    return by_types<Grad>(l.d.table_type, l.d.rows_type, &l, rows, table, err);
 }
 
 }  // namespace accb

@@ -58,7 +58,15 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi)
     return r;
 }
 
+// 16 bytes of x as they were loaded: kept packed until the scale is known, which halves the registers that wait for it
 template <typename T> struct alignas(16) Vec16 { T v[16 / sizeof(T)]; };
+
+// where the second pass converts again what the first has converted, the compiler must not keep the first's fp32 values
+template <typename T> __device__ __forceinline__ void forget(Vec16<T>& w)
+{
+    uint4& u = reinterpret_cast<uint4&>(w);
+    asm volatile("" : "+r"(u.x), "+r"(u.y), "+r"(u.z), "+r"(u.w));
+}
 
 // Groups along the rows of x.  TILE = false: a group is 128 neighbours of a row, taken by 128 * sizeof(T) / 16 threads
 // with one 16-byte load each; a block takes kRowUnits * (threads / group) groups.  TILE = true: a block takes one square tile.
@@ -75,7 +83,7 @@ quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __
     constexpr int kUnits = TILE ? kGroup / kSets : 4;
     __shared__ float warp_max[kRowThreads / 32];
     const int set = threadIdx.x / kPer, part = threadIdx.x % kPer;
-    float v[kUnits][E];
+    Vec16<T> v[kUnits];
     int64_t row[kUnits], col[kUnits];
     bool in[kUnits];
 #pragma unroll
@@ -89,21 +97,13 @@ quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __
             col[u] = (g - row[u] * p.col_blocks) * kGroup + part * E;
         }
         in[u] = row[u] < p.rows && col[u] < p.cols;
+        v[u] = Vec16<T>();
         if constexpr (VEC) {
-            if (in[u]) {
-                const Vec16<T> w = *reinterpret_cast<const Vec16<T>*>(x + row[u] * p.xs0 + col[u]);
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[u][e] = (float)w.v[e];
-            }
+            if (in[u]) v[u] = *reinterpret_cast<const Vec16<T>*>(x + row[u] * p.xs0 + col[u]);
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                if (in[u] && col[u] + e < p.cols) v[u][e] = (float)x[row[u] * p.xs0 + (col[u] + e) * p.xs1];
-                else v[u][e] = 0.0f;
-        }
-        if (!in[u]) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[u][e] = 0.0f;
+                if (in[u] && col[u] + e < p.cols) v[u].v[e] = x[row[u] * p.xs0 + (col[u] + e) * p.xs1];
         }
     }
     float amax[kUnits];
@@ -111,7 +111,8 @@ quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __
     for (int u = 0; u < kUnits; ++u) {
         amax[u] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) amax[u] = fmaxf(amax[u], finite_abs(v[u][e]));
+        for (int e = 0; e < E; ++e) amax[u] = fmaxf(amax[u], finite_abs((float)v[u].v[e]));
+        forget(v[u]);
     }
     if constexpr (TILE) {
         float m = 0.0f;
@@ -142,8 +143,8 @@ quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __
         uint32_t w[E / 4];
 #pragma unroll
         for (int e = 0; e < E; e += 4)
-            w[e / 4] = pack2<E5M2>(scaled(v[u][e], inv), scaled(v[u][e + 1], inv)) |
-                       pack2<E5M2>(scaled(v[u][e + 2], inv), scaled(v[u][e + 3], inv)) << 16;
+            w[e / 4] = pack2<E5M2>(scaled((float)v[u].v[e], inv), scaled((float)v[u].v[e + 1], inv)) |
+                       pack2<E5M2>(scaled((float)v[u].v[e + 2], inv), scaled((float)v[u].v[e + 3], inv)) << 16;
         uint8_t* dst = q + row[u] * p.qs + col[u];
         if constexpr (VEC) {
             if constexpr (E == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
@@ -175,24 +176,18 @@ quantize_across_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* 
     const int64_t row0 = (int64_t)(blockIdx.x % row_blocks) * kRows, col_block = blockIdx.x / row_blocks, col0 = col_block * kGroup;
     const int octet = threadIdx.x % 8, quad = threadIdx.x / 8;                // which E rows, which four columns
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    float v[kSets][4][E];
+    Vec16<T> v[kSets][4];
 #pragma unroll
     for (int z = 0; z < kSets; ++z)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const int64_t r = row0 + z * kStrip + octet * E, k = col0 + quad * 4 + c;
             if constexpr (VEC) {
-                if (k < p.cols && r < p.rows) {
-                    const Vec16<T> w = *reinterpret_cast<const Vec16<T>*>(x + k * p.xs1 + r);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) v[z][c][e] = (float)w.v[e];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) v[z][c][e] = 0.0f;
-                }
+                if (k < p.cols && r < p.rows) v[z][c] = *reinterpret_cast<const Vec16<T>*>(x + k * p.xs1 + r);
+                else v[z][c] = Vec16<T>();
             } else {
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[z][c][e] = (k < p.cols && r + e < p.rows) ? (float)x[k * p.xs1 + r + e] : 0.0f;
+                for (int e = 0; e < E; ++e) v[z][c].v[e] = (k < p.cols && r + e < p.rows) ? x[k * p.xs1 + r + e] : (T)0.0f;
             }
         }
     // maxima of each row over its four columns here, over the warp's sixteen, over the block's 128
@@ -202,11 +197,15 @@ quantize_across_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* 
         for (int e = 0; e < E; ++e) {
             float m = 0.0f;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) m = fmaxf(m, finite_abs(v[z][c][e]));
+            for (int c = 0; c < 4; ++c) m = fmaxf(m, finite_abs((float)v[z][c].v[e]));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
             if (lane < 8) col_max[warp][z * kStrip + octet * E + e] = m;
         }
+#pragma unroll
+    for (int z = 0; z < kSets; ++z)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) forget(v[z][c]);
     __syncthreads();
     float tile_max = 0.0f;
     if constexpr (TILE) {
@@ -231,8 +230,8 @@ quantize_across_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* 
             group_scale(m, p.h, s, inv);
             if (TILE ? threadIdx.x == 0 && z == 0 && e == 0 : quad == 0 && row0 + r < p.rows)
                 scales[(TILE ? (int64_t)(blockIdx.x % row_blocks) : row0 + r) * p.ss0 + col_block * p.ss1] = s;
-            bytes[r * (kPitch / 4) + quad] = pack2<E5M2>(scaled(v[z][0][e], inv), scaled(v[z][1][e], inv)) |
-                                             pack2<E5M2>(scaled(v[z][2][e], inv), scaled(v[z][3][e], inv)) << 16;
+            bytes[r * (kPitch / 4) + quad] = pack2<E5M2>(scaled((float)v[z][0].v[e], inv), scaled((float)v[z][1].v[e], inv)) |
+                                             pack2<E5M2>(scaled((float)v[z][2].v[e], inv), scaled((float)v[z][3].v[e], inv)) << 16;
         }
     __syncthreads();
     const int64_t width = p.cols - col0 < kGroup ? p.cols - col0 : kGroup;

@@ -100,6 +100,12 @@ def test_bad_ids_give_zero_rows_and_are_reported_once():
     with pytest.raises(rt.AccbError, match=r"embedding: 2 token id"):
         rt.synchronize()
     assert got[2].eq(2).all() and got.sum() == 128
+    many = torch.full((3000,), 7, device="cuda")
+    many[5], many[1700], many[2999] = 10, -1, 1 << 33
+    rt.embedding_grad(torch.ones(3000, 64, device="cuda"), many, got)
+    with pytest.raises(rt.AccbError, match=r"embedding: 3 token id"):
+        rt.synchronize()
+    assert got[7].eq(2997).all() and got.sum() == 2997 * 64
     with pytest.raises(rt.AccbError) as e:                                # host arrays: from the call itself
         rt.embedding(np.ones((4, 8), np.float32), np.array([4]), np.zeros((1, 8), np.float32))
     assert e.value.code == rt.ERR_INDEX
@@ -125,15 +131,16 @@ def test_gradient_equals_the_formula(kind, tokens, vocab, dim):
 
 @pytest.mark.parametrize("tg,tt", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "bf16"), ("f16", "f32")])
 @pytest.mark.parametrize("beta,padding", [(0.0, None), (1.0, 2), (-0.5, 0), (1.0, None)])
-def test_gradient_types_beta_padding_and_strides(tg, tt, beta, padding):
-    ids = _ids("zipf", 700, 90, 5)
+@pytest.mark.parametrize("tokens", [700, 1500])                           # both gradient kernels: few tokens, sorted tokens
+def test_gradient_types_beta_padding_and_strides(tokens, tg, tt, beta, padding):
+    ids = _ids("zipf", tokens, 90, 5)
     ids[::50] = 2
-    g = torch.randn(700, 80).to(TYPES[tg])
+    g = torch.randn(tokens, 80).to(TYPES[tg])
     old = torch.randn(90, 80).to(TYPES[tt])
     want, err = _grad_want(g, ids, old, 0.75, beta, padding, 90)
     for pad_cols, lead in ((0, 0), (16, 8), (3, 1)):                      # dense, aligned pitch, unaligned pitch and base
         table = torch.full((90, 80 + pad_cols), 4.0, dtype=TYPES[tt], device="cuda")
-        rows = torch.zeros(700, 80 + pad_cols, dtype=TYPES[tg], device="cuda")
+        rows = torch.zeros(tokens, 80 + pad_cols, dtype=TYPES[tg], device="cuda")
         lead = min(lead, pad_cols)
         table[:, lead:lead + 80] = old.cuda()
         rows[:, lead:lead + 80] = g.cuda()
