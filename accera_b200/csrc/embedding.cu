@@ -46,7 +46,7 @@ struct LookupParams {
 };
 
 constexpr int kLookupBlock = 256;
-constexpr int kLookupUnroll = 4;
+constexpr int kLookupUnroll = 2;
 
 __device__ __forceinline__ int64_t load_id(const void* ids, int64_t t, int id_bytes)
 {
@@ -56,7 +56,7 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int64_t t, int id_by
 // A block moves kLookupBlock * kLookupUnroll neighbouring vectors of the flattened rows, so that short and odd rows
 // fill it as well as long ones; a thread has its kLookupUnroll id -> row chains in flight together.
 template <typename TT, typename TR, int E>
-__global__ void __launch_bounds__(kLookupBlock)
+__global__ void __launch_bounds__(kLookupBlock, 8)
 embedding_kernel(const TT* __restrict__ table, const void* __restrict__ ids, TR* __restrict__ rows, int* __restrict__ status,
                  const LookupParams p)
 {
@@ -246,64 +246,78 @@ __device__ void sort_tokens(const void* ids, int* keys0, int* tokens0, int* keys
     if (lane == 0 && bad) { atomicAdd(status + ST_EMBED_COUNT, bad); status[ST_EMBED_ID] = p.launch_id; }
 }
 
-// What step 1 does beside sorting: words without a token get their final value, zero or beta times the old one.  That is
-// writing most of the table, which HBM bounds, while the sort is bound by latency: clusters 1 .. of the launch do it
-// while cluster 0 sorts.  A CTA owns a run of rows and learns from all ids, in shared memory, which of them have tokens.
+// Words without a token get their final value, zero or beta times the old one, from a kernel of its own that runs beside the
+// sort: it writes most of the table, which HBM bounds, while the sort is bound by latency.  The two are launched with
+// programmatic serialization; the sort starts as soon as every clearing CTA has seen the kernels before it complete, and
+// ends only when the clearing grid has ended, so that what follows the sort follows both.
 struct ClearParams {
     int64_t stride;
     int dim;
     int vec;                     // rows are whole 16-byte vectors, 16-byte aligned
     float beta;
-    int rows_per_cta;
+    int ctas;                    // CTA i owns rows i, i + ctas, ..., so that all CTAs together write one stretch of memory after the other
 };
 
-// seen: (rows_per_cta + 31) / 32 words of shared memory
+// seen: one bit of shared memory for each of the CTA's rows
 template <typename TT, int kThreads>
 __device__ __forceinline__ void clear_rows(TT* table, const void* ids, int part, const SortParams& p, const ClearParams& c, uint32_t* seen)
 {
-    const int64_t first = (int64_t)part * c.rows_per_cta;
-    const int rows = (int)(p.vocab - first < c.rows_per_cta ? p.vocab - first : c.rows_per_cta);
-    if (rows <= 0) return;
+    if (part >= p.vocab) return;
+    const int rows = (p.vocab - part + c.ctas - 1) / c.ctas;
     for (int i = threadIdx.x; i < (rows + 31) / 32; i += kThreads) seen[i] = 0u;
     __syncthreads();
 #pragma unroll 8
     for (int i = threadIdx.x; i < p.n; i += kThreads) {
-        const int64_t id = load_id(ids, i, p.id_bytes), at = id - first;
-        if ((uint64_t)at < (uint64_t)rows && id != p.padding_id) atomicOr(seen + at / 32, 1u << (at % 32));
+        const int64_t id = load_id(ids, i, p.id_bytes);
+        if ((uint64_t)id >= (uint64_t)p.vocab || id == p.padding_id) continue;
+        const uint32_t at = (uint32_t)id / (uint32_t)c.ctas;
+        if ((uint32_t)id - at * (uint32_t)c.ctas == (uint32_t)part) atomicOr(seen + at / 32, 1u << (at % 32));
     }
     __syncthreads();
+    // as many threads side by side as a row has vectors: the CTA writes one stretch of memory after the other
     constexpr int V = 16 / (int)sizeof(TT);
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    for (int r = warp; r < rows; r += kThreads / 32) {
+    const int width = c.vec ? c.dim / V : c.dim;
+    int per_row = 32;
+    while (per_row < 256 && per_row < width) per_row *= 2;
+    const int sub = threadIdx.x / per_row, x = threadIdx.x % per_row;
+#pragma unroll 4
+    for (int r = sub; r < rows; r += kThreads / per_row) {
         if (seen[r / 32] >> (r % 32) & 1u) continue;
-        TT* row = table + (first + r) * c.stride;
-        if (c.beta == 0.0f) {
-            if (c.vec) {
-#pragma unroll 8
-                for (int v = lane; v < c.dim / V; v += 32) __stcs(reinterpret_cast<uint4*>(row) + v, make_uint4(0u, 0u, 0u, 0u));
-            } else {
-                for (int i = lane; i < c.dim; i += 32) row[i] = (TT)0.0f;
-            }
+        TT* row = table + (part + (int64_t)r * c.ctas) * c.stride;
+        if (c.beta != 0.0f) {
+            for (int i = x; i < c.dim; i += per_row) row[i] = (TT)(c.beta * (float)row[i]);
+        } else if (c.vec) {
+            for (int v = x; v < width; v += per_row) reinterpret_cast<uint4*>(row)[v] = make_uint4(0u, 0u, 0u, 0u);
         } else {
-            for (int i = lane; i < c.dim; i += 32) row[i] = (TT)(c.beta * (float)row[i]);
+            for (int i = x; i < c.dim; i += per_row) row[i] = (TT)0.0f;
         }
     }
 }
 
+// Two of these an SM: 524 MB of fp32 rows in 80 us; one of 1024 threads an SM took 130.
+constexpr int kClearThreads = 512, kClearWords = 4096;
+
 template <typename TT>
+__global__ void __launch_bounds__(kClearThreads, 2)
+clear_rows_kernel(const void* __restrict__ ids, TT* __restrict__ table, const SortParams p, const ClearParams c)
+{
+    __shared__ uint32_t seen[kClearWords];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    clear_rows<TT, kClearThreads>(table, ids, (int)blockIdx.x, p, c, seen);
+}
+
+// beside_clear: a clearing grid comes right before this one in the stream (see above)
 __global__ void __launch_bounds__(kSortThreads, 1)
-sort_tokens_kernel(const void* __restrict__ ids, int* keys0, int* tokens0, int* keys1, int* tokens1, int* long_words, TT* __restrict__ table, int* status,
-                   const SortParams p, const ClearParams c)
+sort_tokens_kernel(const void* __restrict__ ids, int* keys0, int* tokens0, int* keys1, int* tokens1, int* long_words, int* status, const SortParams p,
+                   int beside_clear)
 {
     extern __shared__ int smem[];
-    pdl_enter();
-    const int ctas = (int)cluster_size();
-    if ((int)blockIdx.x >= ctas) {
-        clear_rows<TT, kSortThreads>(table, ids, (int)blockIdx.x - ctas, p, c, reinterpret_cast<uint32_t*>(smem));
-        return;
-    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (!beside_clear) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (blockIdx.x == 0 && threadIdx.x == 0) *long_words = 0;
     sort_tokens(ids, keys0, tokens0, keys1, tokens1, status, p, smem);
+    if (beside_clear) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ---------------------------------------------------------------------------------
@@ -316,8 +330,8 @@ sort_tokens_kernel(const void* __restrict__ ids, int* keys0, int* tokens0, int* 
 // of additions is fixed by the sorted list, and only words that are long anyway pay for a second pass.
 
 constexpr int kChunk = 32;
-constexpr int kSumThreads = 256;
-constexpr int kSumUnroll = 8;
+constexpr int kSumThreads = 128;
+constexpr int kSumUnroll = 2;
 
 struct SumParams {
     int n, vocab, dim;
@@ -344,19 +358,21 @@ __device__ __forceinline__ void write_sum(TT* table, int64_t word, int64_t strid
 }
 
 template <typename TT, typename TR, int E>
-__global__ void __launch_bounds__(kSumThreads)
+__global__ void __launch_bounds__(kSumThreads, 16)
 sum_rows_kernel(const TR* __restrict__ rows, const int* __restrict__ keys, const int* __restrict__ tokens, TT* __restrict__ table,
                 float* __restrict__ partial, int* __restrict__ long_words, const SumParams p)
 {
     pdl_enter();
     const int chunk = blockIdx.x / p.slabs, slab = blockIdx.x % p.slabs;
     const int i0 = chunk * kChunk, i1 = min(p.n, i0 + kChunk);
-    __shared__ int key[3 * kChunk], token[2 * kChunk];      // places i0 - kChunk .. and i0 ..
+    __shared__ int key[3 * kChunk + 1];                      // places i0 - kChunk ..
+    __shared__ int64_t row_at[2 * kChunk];                   // places i0 ..: where the token's row begins
     for (int j = threadIdx.x; j < 3 * kChunk; j += kSumThreads) {
         const int i = i0 - kChunk + j;
         key[j] = (i >= 0 && i < p.n) ? keys[i] : -1;
-        if (j >= kChunk) token[j - kChunk] = i < p.n ? tokens[i] : 0;
+        if (j >= kChunk) row_at[j - kChunk] = i < p.n ? (int64_t)tokens[i] * p.rows_stride : 0;
     }
+    if (threadIdx.x == 0) key[3 * kChunk] = -1;
     __syncthreads();
     const int* k = key + kChunk;                             // k[i] = key of place i0 + i
     const int len = i1 - i0;
@@ -389,35 +405,44 @@ sum_rows_kernel(const TR* __restrict__ rows, const int* __restrict__ keys, const
             if (!last_long) last = end;
         }
     }
-    if (threadIdx.x == 0 && slab == 0 && last_long && k_last < p.vocab) long_words[1 + atomicAdd(long_words, 1)] = chunk;
+    last_long = last_long && k_last < p.vocab;
+    if (threadIdx.x == 0 && slab == 0 && last_long) long_words[1 + atomicAdd(long_words, 1)] = chunk;
+    // ids that stand for no word come last
+    const int valid = __popc(__ballot_sync(0xffffffffu, (uint32_t)k[lane] < (uint32_t)p.vocab)) +
+                      __popc(__ballot_sync(0xffffffffu, (uint32_t)k[lane + kChunk] < (uint32_t)p.vocab));
+    last = min(last, valid);
+    // places whose word ends there, the next one being another's
+    const uint64_t ends = (uint64_t)__ballot_sync(0xffffffffu, k[lane] != k[lane + 1]) | (uint64_t)__ballot_sync(0xffffffffu, k[lane + kChunk] != k[lane + kChunk + 1]) << 32;
     const int col = (slab * kSumThreads + threadIdx.x) * E;
-    if (col >= p.dim) return;
+    if (col >= p.dim || first >= last) return;
+    // kSumUnroll rows are always on their way: a place's register takes the row kSumUnroll places on as soon as it is added
+    const TR* src = rows + col;
+    Vec<TR, E> x[kSumUnroll];
+#pragma unroll
+    for (int u = 0; u < kSumUnroll; ++u) x[u] = *reinterpret_cast<const Vec<TR, E>*>(src + row_at[min(first + u, last - 1)]);
     float acc[E] = {};
     for (int j0 = first; j0 < last; j0 += kSumUnroll) {
-        Vec<TR, E> x[kSumUnroll];
-#pragma unroll
-        for (int u = 0; u < kSumUnroll; ++u)
-            if (j0 + u < last && k[j0 + u] < p.vocab)
-                x[u] = *reinterpret_cast<const Vec<TR, E>*>(rows + (int64_t)token[j0 + u] * p.rows_stride + col);
 #pragma unroll
         for (int u = 0; u < kSumUnroll; ++u) {
             const int j = j0 + u;
-            if (j < last && k[j] < p.vocab) {
+            if (j >= last) break;
 #pragma unroll
-                for (int e = 0; e < E; ++e) acc[e] += (float)x[u].v[e];
-                const bool ends = j + 1 == last || k[j + 1] != k[j];
-                if (ends) {
-                    const bool head = first_long && k[j] == k[0], tail = last_long && j + 1 == last;
-                    if (head || tail) {
-                        float* dst = partial + ((int64_t)chunk * 2 + (head ? 0 : 1)) * p.dim + col;
+            for (int e = 0; e < E; ++e) acc[e] += (float)x[u].v[e];
+            if (j + kSumUnroll < last) x[u] = *reinterpret_cast<const Vec<TR, E>*>(src + row_at[j + kSumUnroll]);
+            if (j + 1 == last || (ends >> j & 1u)) {
+                const bool head = first_long && k[j] == k_first, tail = last_long && j + 1 == last;
+                if (head || tail) {
+                    Vec<float, E> y;
 #pragma unroll
-                        for (int e = 0; e < E; ++e) dst[e] = acc[e];
-                    } else {
-                        write_sum<TT, E>(table, k[j], p.table_stride, col, acc, p.scale, p.beta);
-                    }
-#pragma unroll
-                    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+                    for (int e = 0; e < E; ++e) y.v[e] = acc[e];
+                    float* dst = partial + ((int64_t)chunk * 2 + (head ? 0 : 1)) * p.dim + col;
+                    if constexpr (E == 1) *dst = acc[0];
+                    else *reinterpret_cast<Vec<float, E>*>(dst) = y;
+                } else {
+                    write_sum<TT, E>(table, k[j], p.table_stride, col, acc, p.scale, p.beta);
                 }
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] = 0.0f;
             }
         }
     }
@@ -426,20 +451,20 @@ sum_rows_kernel(const TR* __restrict__ rows, const int* __restrict__ keys, const
 // step 3: the pieces of the long words.  long_words[0] of them begin in chunks long_words[1 ..] (in any order: each is a sum
 // of its own).  A block takes kJoinCols columns of one word at a time: kJoinLanes threads a column add every kJoinLanes-th
 // piece, and their sums are added in lane order.
-constexpr int kJoinCols = 32, kJoinLanes = 16;
+constexpr int kJoinCols = 32, kJoinLanes = 8;
 
-template <typename TT>
+template <typename TT, int E>
 __global__ void __launch_bounds__(kJoinCols * kJoinLanes)
 join_rows_kernel(const float* __restrict__ partial, const int* __restrict__ keys, const int* __restrict__ long_words, TT* __restrict__ table,
                  const SumParams p)
 {
     pdl_enter();
-    __shared__ float part[kJoinLanes][kJoinCols];
+    __shared__ Vec<float, E> part[kJoinLanes][kJoinCols];
     const int x = threadIdx.x % kJoinCols, y = threadIdx.x / kJoinCols;
-    const int col_blocks = (p.dim + kJoinCols - 1) / kJoinCols;
+    const int col_blocks = (p.dim + kJoinCols * E - 1) / (kJoinCols * E);
     const int64_t total = (int64_t)long_words[0] * col_blocks;
     for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
-        const int chunk = long_words[1 + w / col_blocks], col = (int)(w % col_blocks) * kJoinCols + x;
+        const int chunk = long_words[1 + w / col_blocks], col = ((int)(w % col_blocks) * kJoinCols + x) * E;
         const int word = keys[chunk * kChunk + kChunk - 1];
         // the first place behind the word, found by each warp for itself with 32 probes a step of the sorted list
         int lo = chunk * kChunk + kChunk, hi = p.n;
@@ -452,19 +477,24 @@ join_rows_kernel(const float* __restrict__ partial, const int* __restrict__ keys
             if (inside > 0) lo += (inside - 1) * step + 1;
         }
         const int last_chunk = (lo - 1) / kChunk;
-        float acc = 0.0f;
+        Vec<float, E> acc = {};
         if (col < p.dim) {
-#pragma unroll 4
-            for (int c = chunk + y; c <= last_chunk; c += kJoinLanes)
-                acc += __ldcs(partial + ((int64_t)c * 2 + (c == chunk ? 1 : 0)) * p.dim + col);
+#pragma unroll 8
+            for (int c = chunk + y; c <= last_chunk; c += kJoinLanes) {
+                const Vec<float, E> v = *reinterpret_cast<const Vec<float, E>*>(partial + ((int64_t)c * 2 + (c == chunk ? 1 : 0)) * p.dim + col);
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc.v[e] += v.v[e];
+            }
         }
         part[y][x] = acc;
         __syncthreads();
         if (y == 0 && col < p.dim) {
-            float sum[1] = { 0.0f };
+            float sum[E] = {};
 #pragma unroll
-            for (int l = 0; l < kJoinLanes; ++l) sum[0] += part[l][x];
-            write_sum<TT, 1>(table, word, p.table_stride, col, sum, p.scale, p.beta);
+            for (int l = 0; l < kJoinLanes; ++l)
+#pragma unroll
+                for (int e = 0; e < E; ++e) sum[e] += part[l][x].v[e];
+            write_sum<TT, E>(table, word, p.table_stride, col, sum, p.scale, p.beta);
         }
         __syncthreads();
     }
@@ -582,8 +612,29 @@ ClearParams clear_params(const accb_embedding_desc& d, const void* table, int64_
     ClearParams c;
     c.stride = d.table_stride; c.dim = (int)d.dim; c.beta = d.beta;
     c.vec = (d.dim * sizeof(TT)) % 16 == 0 && (d.table_stride * sizeof(TT)) % 16 == 0 && (reinterpret_cast<uintptr_t>(table) & 15) == 0;
-    c.rows_per_cta = (int)((d.vocab + ctas - 1) / ctas);
+    c.ctas = (int)ctas;
     return c;
+}
+
+cudaError_t launch_sort(const EmbeddingLaunch& l, const SortParams& s, int* keys0, int* tokens0, int* keys1, int* tokens1, int* long_words, bool beside_clear)
+{
+    static std::atomic<bool> opted[64];
+    if (l.device >= 64 || !opted[l.device].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(sort_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSortSmem);
+        if (e != cudaSuccess) return e;
+        if (l.device < 64) opted[l.device].store(true, std::memory_order_release);
+    }
+    const unsigned cluster = s.n <= 2048 ? 1 : s.n <= 4096 ? 2 : s.n <= 8192 ? 4 : kSortCluster;
+    const bool pdl = options().stream_pdl != 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cluster); cfg.blockDim = dim3(kSortThreads); cfg.dynamicSmemBytes = kSortSmem; cfg.stream = l.stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, sort_tokens_kernel, l.ids, keys0, tokens0, keys1, tokens1, long_words, l.status, s, beside_clear ? 1 : 0);
 }
 
 template <typename TT, typename TR>
@@ -606,8 +657,7 @@ int launch_grad(const EmbeddingLaunch& l, const void* rows, void* table, const c
     p.table_stride = d.table_stride; p.rows_stride = d.rows_stride;
     p.scale = d.scale; p.beta = d.beta;
     p.chunks = (int)((n + kChunk - 1) / kChunk);
-    static_assert(kSumThreads == kFewThreads, "one slab width");
-    const int64_t cols_per_slab = (int64_t)kSumThreads * (vec ? E : 1);
+    const int64_t cols_per_slab = (int64_t)(n <= kFewTokens ? kFewThreads : kSumThreads) * (vec ? E : 1);
     p.slabs = (int)((d.dim + cols_per_slab - 1) / cols_per_slab);
     auto cuda_failed = [&](cudaError_t e) { *err = cudaGetErrorString(e); return (int)ACCB_ERR_CUDA; };
 
@@ -636,40 +686,23 @@ int launch_grad(const EmbeddingLaunch& l, const void* rows, void* table, const c
     const int* keys = (s.passes & 1) ? keys0 : keys1;
     const int* tokens = (s.passes & 1) ? tokens0 : tokens1;
     cudaError_t e = cudaSuccess;
-    {
-        auto kernel = sort_tokens_kernel<TT>;
-        static std::atomic<bool> opted[64];
-        if (l.device >= 64 || !opted[l.device].load(std::memory_order_acquire)) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSortSmem);
-            if (e == cudaSuccess && l.device < 64) opted[l.device].store(true, std::memory_order_release);
-        }
-        const int cluster = n <= 2048 ? 1 : n <= 4096 ? 2 : n <= 8192 ? 4 : kSortCluster;
-        // one clearing CTA an SM beside the sorting cluster; more only where a CTA's bit list (its shared memory) ends
-        const int64_t most = (int64_t)(kSortSmem / 4) * 32, need = (d.vocab + most - 1) / most;
-        int64_t ctas = clear ? (l.num_sms - cluster) / cluster * cluster : 0;
-        if (clear && need > ctas) ctas = (need + cluster - 1) / cluster * cluster;
-        const ClearParams c = clear_params<TT>(d, table, ctas > 0 ? ctas : 1);
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(cluster + ctas)); cfg.blockDim = dim3(kSortThreads); cfg.dynamicSmemBytes = kSortSmem; cfg.stream = l.stream;
-        cudaLaunchAttribute attr[2];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = (unsigned)cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[1].val.programmaticStreamSerializationAllowed = options().stream_pdl == 0 ? 0 : 1;
-        cfg.attrs = attr; cfg.numAttrs = 2;
-        if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, l.ids, keys0, tokens0, keys1, tokens1, long_words, (TT*)table, l.status, s, c);
+    if (clear) {
+        const int64_t most = (int64_t)kClearWords * 32, need = (d.vocab + most - 1) / most;
+        const int64_t ctas = need > 2 * l.num_sms ? need : 2 * l.num_sms;
+        e = launch_pdl(clear_rows_kernel<TT>, dim3((unsigned)ctas), dim3(kClearThreads), l.stream, l.ids, (TT*)table, s, clear_params<TT>(d, table, ctas));
     }
+    if (e == cudaSuccess) e = launch_sort(l, s, keys0, tokens0, keys1, tokens1, long_words, clear);
     const dim3 grid((unsigned)blocks), block(kSumThreads);
     if (e == cudaSuccess)
         e = vec ? launch_pdl(sum_rows_kernel<TT, TR, E>, grid, block, l.stream, (const TR*)rows, keys, tokens, (TT*)table, partial, long_words, p)
                 : launch_pdl(sum_rows_kernel<TT, TR, 1>, grid, block, l.stream, (const TR*)rows, keys, tokens, (TT*)table, partial, long_words, p);
     if (e == cudaSuccess)
-        e = launch_pdl(join_rows_kernel<TT>, dim3((unsigned)(4 * l.num_sms)), dim3(kJoinCols * kJoinLanes), l.stream, (const float*)partial, keys,
-                       (const int*)long_words, (TT*)table, p);
+        e = launch_pdl(vec ? join_rows_kernel<TT, 4> : join_rows_kernel<TT, 1>, dim3((unsigned)(8 * l.num_sms)), dim3(kJoinCols * kJoinLanes), l.stream,
+                       (const float*)partial, keys, (const int*)long_words, (TT*)table, p);
     temp_free(ws, l.stream);
     if (e != cudaSuccess) return cuda_failed(e);
-    note_launches(3);
-    return 3;
+    note_launches(clear ? 4 : 3);
+    return clear ? 4 : 3;
 }
 
 template <template <typename, typename> class F, typename... Args>
