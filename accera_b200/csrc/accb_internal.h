@@ -127,7 +127,7 @@ void gemm_umma_launch_geometry(const GemmLaunch& g, int want_two_sm, int32_t out
 
 // gemm_splitk.cu: C <- epi(alpha * sum of `slices` dense row-major M x N partials (fp32, or int32 for an int32 C) + beta * C + bias)
 int launch_splitk_reduce(const void* partial, int slices, const accb_gemm_desc& d, void* c, const float* bias,
-                         cudaStream_t stream, const char** err);
+                         cudaStream_t stream, const char** err, bool relu_keeps_nan = false);
 
 // repack.cu: copy of an operand into rows with a 16-byte aligned pitch, zero-padded (see the file)
 int launch_repack_rows(const void* src, int64_t src_pitch, int64_t rows, int64_t width, int elem_bytes, void* dst,

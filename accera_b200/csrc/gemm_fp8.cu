@@ -14,8 +14,9 @@
 //          MMAs without the additions take 397 us, so the loop is bound by the round trip of a TMEM buffer (MMAs done -
 //          read by both CTAs' warps - MMA issued again), of which only two fit TMEM at this width.  Narrower tiles with
 //          three or four buffers (160, 128 columns) were measured slower, 650 and 700 us: their operands alone take 500 and 540.
-//   tile   128 x BN tiles by single CTAs for problems with too few large tiles: columns of C (weights) on the 128 TMEM
-//          lanes, rows of C (tokens) on BN = 16 .. 128 accumulator columns, K cut into up to eight slices
+//          Problems with few tiles cut K into slices, whose fp32 sums gemm_splitk.cu adds in slice order.
+//   tile   128 x BN tiles by single CTAs for up to 64 rows of C: columns of C (weights) on the 128 TMEM
+//          lanes, rows of C (tokens) on BN = 16 .. 64 accumulator columns, K cut into up to eight slices
 //          that a cluster multiplies side by side and adds, slice by slice, through distributed shared memory.
 // Scales reach shared memory by 4-byte cp.async (any strides), eight blocks ahead, by the warp that also issues the TMA loads.
 //
@@ -53,7 +54,8 @@ struct F8Params {
     int num_kb;
     uint32_t idesc;
     int tiles_m, tiles_n, group_m;
-    int slices;                             // tile kernel: CTAs of a cluster that share one tile's K
+    int slices;                             // parts that K is cut into: CTAs of a cluster (tile kernel), work items (pair kernel)
+    int64_t slice_stride;                   // pair kernel: elements of C from one slice's sums to the next's
     int c_mode;                             // pair kernel: 2 rows of 16-byte vectors, 1 contiguous rows, 0 any strides
     int* status;
     int launch_id;
@@ -139,10 +141,10 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ float load_cluster(uint32_t addr)
+__device__ __forceinline__ float4 load_cluster4(uint32_t addr)
 {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
     return v;
 }
 
@@ -292,8 +294,17 @@ __device__ __forceinline__ void store_box(float (&v)[128 / sizeof(TC)], uint8_t*
     __syncwarp();
 }
 
-__device__ __forceinline__ void pair_tile(int t, const F8Params& p, int& tm, int& tn)
+// work item -> tile and range of blocks of K
+template <bool SPLIT>
+__device__ __forceinline__ void pair_item(int t, const F8Params& p, int& tm, int& tn, int& slice, int& kb_begin, int& kb_end)
 {
+    slice = 0; kb_begin = 0; kb_end = p.num_kb;
+    if (SPLIT) {
+        slice = t % p.slices;
+        t /= p.slices;
+        kb_begin = (int)((int64_t)p.num_kb * slice / p.slices);
+        kb_end = (int)((int64_t)p.num_kb * (slice + 1) / p.slices);
+    }
     const int group_size = p.group_m * p.tiles_n;
     const int group = t / group_size;
     const int first_m = group * p.group_m;
@@ -320,8 +331,8 @@ __device__ __forceinline__ void add_scaled(float* acc, const uint32_t (&x)[32], 
     }
 }
 
-// COLS: every column of B has a scale of its own (else 128 share one)
-template <typename TC, bool COLS>
+// COLS: every column of B has a scale of its own (else 128 share one).  SPLIT: K is cut into slices, C holds their sums.
+template <typename TC, bool COLS, bool SPLIT>
 __global__ void __launch_bounds__(PairPlan::kThreads, 1)
 gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, TC* __restrict__ C, const F8Params p)
 {
@@ -371,9 +382,8 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     const uint32_t tmem_base = *tmem_holder;
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    const int num_tiles = p.tiles_m * p.tiles_n;
+    const int num_tiles = p.tiles_m * p.tiles_n * (SPLIT ? p.slices : 1);
     const int num_units = (int)gridDim.x / 2, unit = (int)blockIdx.x / 2;
-    const int num_kb = p.num_kb;
 
     if (warp < Plan::kEpilogueWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Plan::kFewRegisters));
@@ -384,10 +394,10 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             uint32_t ph = 0;
             bool ok = true;
             for (int t = unit; t < num_tiles && ok; t += num_units) {
-                int tm, tn;
-                pair_tile(t, p, tm, tn);
+                int tm, tn, slice, kb_begin, kb_end;
+                pair_item<SPLIT>(t, p, tm, tn, slice, kb_begin, kb_end);
                 const int row_a = (tm * 2 + (int)rank) * kRowsX, row_b = tn * Plan::kBN + (int)rank * 128;
-                for (int kb = 0; kb < num_kb; ++kb) {
+                for (int kb = kb_begin; kb < kb_end; ++kb) {
                     if (!mbar_wait(done_bar(s), ph ^ 1u, wctx, SITE_PRODUCER_EMPTY, kb)) { ok = false; break; }
                     const uint32_t sa = smem_base + s * Plan::kStageBytes, sb = sa + kRowsX * kSlabBytes;
                     if (leader) mbar_arrive_expect_tx(full_bar(s), 2u * Plan::kStageBytes);
@@ -406,13 +416,13 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         uint32_t rph = 0;
         bool ok = true;
         for (int t = unit; t < num_tiles && ok; t += num_units) {
-            int tm, tn;
-            pair_tile(t, p, tm, tn);
+            int tm, tn, slice, kb_begin, kb_end;
+            pair_item<SPLIT>(t, p, tm, tn, slice, kb_begin, kb_end);
             const int64_t row_a = (int64_t)(tm * 2 + (int)rank) * kRowsX + lane, col_b = (int64_t)tn * Plan::kBN + lane * (COLS ? 1 : 128);
-            for (int kb0 = 0; kb0 < num_kb; kb0 += Plan::kGroup) {
+            for (int kb0 = kb_begin; kb0 < kb_end; kb0 += Plan::kGroup) {
                 ok = __all_sync(0xffffffffu, mbar_wait(scale_empty_bar(r), rph ^ 1u, wctx, SITE_PRODUCER_EMPTY, kb0));
                 if (!ok) break;
-                const int blocks = min(Plan::kGroup, num_kb - kb0);
+                const int blocks = min(Plan::kGroup, kb_end - kb0);
                 for (int j = 0; j < blocks; ++j) {
                     const uint32_t sc = smem_base + Plan::kScales + (r * Plan::kGroup + j) * Plan::kScaleBytes;
                     const float* sa = p.sa + (kb0 + j) * p.sa_kb;
@@ -439,7 +449,12 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         if (leader) {
             const uint64_t a0 = operand_desc(smem_base, p.a_mn), b0 = operand_desc(smem_base + kRowsX * kSlabBytes, p.b_mn);
             const uint32_t a_step = operand_step(p.a_mn), b_step = operand_step(p.b_mn), elected = elect_lane();
-            const int blocks = (num_tiles - unit + num_units - 1) / num_units * num_kb;
+            int blocks = 0;
+            for (int t = unit; t < num_tiles; t += num_units) {
+                int tm, tn, slice, kb_begin, kb_end;
+                pair_item<SPLIT>(t, p, tm, tn, slice, kb_begin, kb_end);
+                blocks += kb_end - kb_begin;
+            }
             int s = 0;
             uint32_t ph = 0;
             bool ok = true;
@@ -469,8 +484,8 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         uint32_t rph = 0, ph = 0;
         bool ok = true;
         for (int t = unit; t < num_tiles && ok; t += num_units) {
-            int tm, tn;
-            pair_tile(t, p, tm, tn);
+            int tm, tn, slice, kb_begin, kb_end;
+            pair_item<SPLIT>(t, p, tm, tn, slice, kb_begin, kb_end);
             float acc[128];
 #pragma unroll
             for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
@@ -478,6 +493,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             // before the last of the block before it is added, if that block's MMAs are done by then.
             uint32_t x0[32], x1[32];
             bool loading = false;
+            const int num_kb = SPLIT ? kb_end - kb_begin : p.num_kb;
             for (int kb = 0; kb < num_kb; ++kb, ++g) {
                 const int buf = g & 1, in_group = kb % Plan::kGroup;
                 const uint32_t taddr = taddr0 + (uint32_t)(buf * Plan::kBN);
@@ -546,7 +562,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 float v[W];
 #pragma unroll
                 for (int j = 0; j < W; ++j) v[j] = acc[b * W + j];
-                if (row0 < p.m && col0 + b * W < p.n) store_box<TC>(v, box, C, row0, col0 + b * W, lane, p);
+                if (row0 < p.m && col0 + b * W < p.n) store_box<TC>(v, box, SPLIT ? C + slice * p.slice_stride : C, row0, col0 + b * W, lane, p);
             }
         }
         if (!ok && lane == 0) record_give_up();
@@ -573,8 +589,8 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
 template <int BN> struct TilePlan {
     static constexpr int kThreads = 192;                                 // TMA + scales, MMA, four epilogue warps
     static constexpr int kStageBytes = (kRowsX + BN) * kSlabBytes;       // 128 columns of C (weights), BN rows of C (tokens)
-    static constexpr int kStages = BN == 128 ? 3 : BN == 64 ? 4 : BN == 32 ? 5 : 5;
-    static constexpr int kBuffers = BN == 128 ? 2 : BN == 64 ? 4 : 8;    // TMEM accumulators of BN columns
+    static constexpr int kStages = BN == 64 ? 4 : 5;
+    static constexpr int kBuffers = BN == 64 ? 4 : 8;    // TMEM accumulators of BN columns
     static constexpr int kTmemCols = kBuffers * BN;
     static constexpr int kScaleBytes = (kRowsX + BN) * 4;
     static constexpr int kScales = kStages * kStageBytes;
@@ -666,8 +682,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                     mbar_arrive_expect_tx(full_bar(s), (uint32_t)Plan::kStageBytes);
                     if (p.b_mn) tma_load_2d(sw, &map_w, full_bar(s), row0, kb * kSlabBytes, 0);
                     else tma_load_2d(sw, &map_w, full_bar(s), kb * kSlabBytes, row0, 0);
-                    if (p.a_mn) tma_load_2d(st, &map_t, full_bar(s), col0, kb * kSlabBytes, 0);
-                    else tma_load_2d(st, &map_t, full_bar(s), kb * kSlabBytes, col0, 0);
+                    tma_load_2d(st, &map_t, full_bar(s), kb * kSlabBytes, col0, 0);
                 }
             }
             if (++s == S) { s = 0; ph ^= 1u; }
@@ -704,12 +719,8 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                     if (++b == NB) { b = 0; bph ^= 1u; }
                 }
             };
-            if (!p.b_mn && !p.a_mn) issue(std::false_type{}, std::false_type{});
-            else if (!p.a_mn) issue(std::true_type{}, std::false_type{});
-            else if constexpr (BN == 128) {                              // an M-contiguous box is 128 wide: the host takes BN = 128 then
-                if (!p.b_mn) issue(std::false_type{}, std::true_type{});
-                else issue(std::true_type{}, std::true_type{});
-            }
+            if (!p.b_mn) issue(std::false_type{}, std::false_type{});
+            else issue(std::true_type{}, std::false_type{});
         }
     } else {
         const int q = warp & 3;
@@ -760,9 +771,10 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     }
 
     // All loads and MMAs of this CTA are done: the operand ring may hold the slice's sums, [BN][128] fp32.
-    const int64_t n_index = (int64_t)row0 + (warp & 3) * 32 + lane;
-    const int cols = (int)(p.m - col0 < BN ? p.m - col0 : BN);
-    auto put = [&](int c, float v) {
+    const int cols = (int)(p.m - col0 < BN ? p.m - col0 : BN), at = (warp & 3) * 32 + lane;
+    // element (token c of the tile, weight r of the tile)
+    auto put = [&](int c, int r, float v) {
+        const int64_t n_index = (int64_t)row0 + r;
         if (n_index >= p.n) return;
         TC* d = C + (col0 + c) * p.cs0 + n_index * p.cs1;
         *d = (TC)finish(v, p.beta != 0.0f ? (float)*d : 0.0f, p.bias ? __ldg(p.bias + n_index) : 0.0f, p);
@@ -773,14 +785,13 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             for (int c = 0; c < BN; c += 2) {
                 float lo, hi;
                 unpack2(acc[c / 2], lo, hi);
-                if (c < cols) put(c, lo);
-                if (c + 1 < cols) put(c + 1, hi);
+                if (c < cols) put(c, at, lo);
+                if (c + 1 < cols) put(c + 1, at, hi);
             }
         }
         return;
     }
     float* sums = reinterpret_cast<float*>(smem_gen);
-    const int at = (warp & 3) * 32 + lane;
     if (warp >= 2) {
 #pragma unroll
         for (int c = 0; c < BN; c += 2) {
@@ -792,11 +803,28 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     }
     cluster_sync_all();
     if (warp >= 2) {
-        // this CTA's share of the columns: every slices-th, the slices' sums added in their order along K
-        for (int c = slice; c < cols; c += p.slices) {
-            float v = 0.0f;
-            for (int z = 0; z < p.slices; ++z) v += load_cluster(map_to_rank(smem_base + (uint32_t)(c * kRowsX + at) * 4, (uint32_t)z));
-            put(c, v);
+        // This CTA's share of the columns: every slices-th, one a warp at a time, four weights a lane; the slices' sums are
+        // added in their order along K.  Reads from other CTAs take long, so those of two columns are issued together.
+        const int step = p.slices * 4;
+        for (int c = slice + p.slices * (warp - 2); c < cols; c += 2 * step) {
+            float4 v[2] = {};
+            const bool two = c + step < cols;
+#pragma unroll 4
+            for (int z = 0; z < p.slices; ++z) {
+                const uint32_t other = map_to_rank(smem_base + (uint32_t)(c * kRowsX + lane * 4) * 4, (uint32_t)z);
+                const float4 a = load_cluster4(other);
+                const float4 b = load_cluster4(two ? other + (uint32_t)(step * kRowsX) * 4 : other);
+                v[0].x += a.x; v[0].y += a.y; v[0].z += a.z; v[0].w += a.w;
+                v[1].x += b.x; v[1].y += b.y; v[1].z += b.z; v[1].w += b.w;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (h == 1 && !two) break;
+                put(c + h * step, lane * 4, v[h].x);
+                put(c + h * step, lane * 4 + 1, v[h].y);
+                put(c + h * step, lane * 4 + 2, v[h].z);
+                put(c + h * step, lane * 4 + 3, v[h].w);
+            }
         }
     }
     cluster_sync_all();                                                  // nobody leaves while its sums are being read
@@ -822,10 +850,10 @@ uint32_t f8_idesc(const accb_gemm_desc& d, bool swapped, int m, int n, bool a_mn
 
 constexpr int kMaxDevices = 64;
 
-template <typename TC, bool COLS>
+template <typename TC, bool COLS, bool SPLIT>
 cudaError_t launch_pair(const GemmFp8Launch& g, const CUtensorMap& ma, const CUtensorMap& mb, const F8Params& p)
 {
-    auto kernel = gemm_fp8_pair_kernel<TC, COLS>;
+    auto kernel = gemm_fp8_pair_kernel<TC, COLS, SPLIT>;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(PairPlan::kThreads);
     cfg.dynamicSmemBytes = PairPlan::kTotal;
@@ -849,7 +877,7 @@ cudaError_t launch_pair(const GemmFp8Launch& g, const CUtensorMap& ma, const CUt
         if (g.device < kMaxDevices) resident[g.device].store(units, std::memory_order_release);
     }
     if (g.d.max_ctas > 0 && units > (g.d.max_ctas + 1) / 2) units = (g.d.max_ctas + 1) / 2;
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.slices;
     if (units > tiles) units = (int)tiles;
     cfg.gridDim = dim3((unsigned)(2 * units));
     return cudaLaunchKernelEx(&cfg, kernel, ma, mb, (TC*)g.c, p);
@@ -882,8 +910,11 @@ cudaError_t launch_tile(const GemmFp8Launch& g, const CUtensorMap& mw, const CUt
 template <typename TC>
 cudaError_t launch_c(const GemmFp8Launch& g, const CUtensorMap& ma, const CUtensorMap& mb, const F8Params& p, int bn)
 {
-    if (bn == 256) return p.b_shift ? launch_pair<TC, false>(g, ma, mb, p) : launch_pair<TC, true>(g, ma, mb, p);
-    if (bn == 128) return launch_tile<TC, 128>(g, mb, ma, p);
+    if (bn == 256) {
+        if constexpr (std::is_same<TC, float>::value)
+            if (p.slices > 1) return p.b_shift ? launch_pair<TC, false, true>(g, ma, mb, p) : launch_pair<TC, true, true>(g, ma, mb, p);
+        return p.b_shift ? launch_pair<TC, false, false>(g, ma, mb, p) : launch_pair<TC, true, false>(g, ma, mb, p);
+    }
     if (bn == 64) return launch_tile<TC, 64>(g, mb, ma, p);
     if (bn == 32) return launch_tile<TC, 32>(g, mb, ma, p);
     return launch_tile<TC, 16>(g, mb, ma, p);
@@ -943,24 +974,59 @@ int launch_gemm_fp8(const GemmFp8Launch& g0, const char** err)
     const Options& o = options();
     p.wait_ns = o.gemm_wait_limit_us > 0 ? (unsigned long long)o.gemm_wait_limit_us * 1000ull : 1000000000ull;
 
-    const int64_t pair_tiles = ((d.m + 255) / 256) * ((d.n + 255) / 256);
-    bool pair = d.max_ctas > 0 || (d.m > 128 && pair_tiles * 2 > g.num_sms / 2);
+    // Which kernel, and how many slices of K, by estimated microseconds, fitted to measured launches (graph replays).
+    //   pair   a round of tiles takes 0.55 a block of K and 6 at its ends; slices add a second pass: 6, and its bytes at 4 TB/s
+    //   tile   a wave of CTAs (two an SM) takes 0.6, 0.7, 0.9 a block for 16, 32, 64 rows, two thirds of it with one CTA an SM;
+    //          4 at its ends and 1, 2, 3 more for the sum over a cluster, which only pays within one wave
+    // For example 64 x 4096 x 4096: tile with 8 slices 10.4, pair at best 19; 256 x 4096 x 4096: 19 and 20.6; 128 x 32000 x 4096: 62 and 49.
+    const int64_t pair_tiles = ((d.m + 255) / 256) * ((d.n + 255) / 256), pair_units = g.num_sms / 2;
+    auto pair_cost = [&](int64_t sl) {
+        return (double)((pair_tiles * sl + pair_units - 1) / pair_units) * ((double)((p.num_kb + sl - 1) / sl) * 0.55 + 6.0) +
+               (sl > 1 ? 6.0 + (double)(sl + 1) * (double)d.m * (double)d.n * 4.0 / 4.0e6 : 0.0);
+    };
+    int pair_slices = 1;
+    for (int sl = 2; sl <= 16 && pair_tiles * sl <= pair_units && sl * 2 <= p.num_kb; ++sl)
+        if (pair_cost(sl) < 0.95 * pair_cost(pair_slices)) pair_slices = sl;
+    const int tile_bn = d.m <= 16 ? 16 : d.m <= 32 ? 32 : 64;
+    const int64_t tiles = ((d.m + tile_bn - 1) / tile_bn) * ((d.n + kRowsX - 1) / kRowsX);
+    auto tile_cost = [&](int64_t sl) {
+        const int64_t ctas = tiles * sl;
+        const double block = (tile_bn == 16 ? 0.6 : tile_bn == 32 ? 0.7 : 0.9) * (ctas <= g.num_sms ? 0.65 : 1.0);
+        return (double)((ctas + 2 * g.num_sms - 1) / (2 * g.num_sms)) * (double)((p.num_kb + sl - 1) / sl) * block + 4.0 + (sl > 1 ? (tile_bn == 16 ? 1.0 : tile_bn == 32 ? 2.0 : 3.0) : 0.0);
+    };
+    int tile_slices = 1;
+    for (int sl = 2; sl <= 8 && sl <= p.num_kb && tiles * sl <= 2 * g.num_sms; sl *= 2)
+        if (tile_cost(sl) < tile_cost(tile_slices)) tile_slices = sl;
+    bool pair = pair_cost(pair_slices) <= tile_cost(tile_slices);
     if (o.gemm_fp8_kernel) pair = o.gemm_fp8_kernel == 1;
+    if (d.max_ctas > 0 || a_dir == 1) pair = true;      // persistent; and the tile kernel takes no A that is contiguous along M
     int bn = 256;
+    GemmFp8Launch part = g;                  // what the kernel computes: g, or the fp32 sums of the slices of K
+    void* sums = nullptr;
     if (pair) {
         p.tiles_m = (int)((d.m + 255) / 256); p.tiles_n = (int)((d.n + 255) / 256);
         p.group_m = 8;
         p.idesc = f8_idesc(d, false, 256, 256, a_dir, b_dir);
-        const int es = elem_size(d.c_type);
-        p.c_mode = d.c_stride[1] != 1 ? 0 : (d.c_stride[0] * es % 16 == 0 && (reinterpret_cast<uintptr_t>(g.c) & 15) == 0) ? 2 : 1;
-        if (pair_tiles > 0x3fffffff) { release(); *err = "too many tiles"; return ACCB_ERR_ARG; }
+        if (pair_tiles > 0x3ffffff) { release(); *err = "too many tiles"; return ACCB_ERR_ARG; }
+        // with a bounded grid the units are fewer than the estimate's
+        int slices = d.max_ctas > 0 ? 1 : pair_slices;
+        if (o.gemm_fp8_slices > 0) slices = o.gemm_fp8_slices < p.num_kb ? o.gemm_fp8_slices : p.num_kb;
+        if (slices > 1) sums = temp_alloc(g.device, (size_t)slices * (size_t)d.m * (size_t)d.n * 4, g.stream);
+        p.slices = sums ? slices : 1;        // (no memory to spare: one slice)
+        if (sums) {
+            p.slice_stride = d.m * d.n;
+            p.cs0 = d.n; p.cs1 = 1;
+            p.alpha = 1.0f; p.beta = 0.0f; p.bias = nullptr; p.relu = 0;
+            part.c = sums;
+            part.d.c_type = ACCB_F32;
+        }
+        const int es = elem_size(part.d.c_type);
+        p.c_mode = p.cs1 != 1 ? 0 : (p.cs0 * es % 16 == 0 && (reinterpret_cast<uintptr_t>(part.c) & 15) == 0 && p.slice_stride * es % 16 == 0) ? 2 : 1;
     } else {
-        bn = a_dir ? 128 : d.m <= 16 ? 16 : d.m <= 32 ? 32 : d.m <= 64 ? 64 : 128;
+        bn = tile_bn;
         p.tiles_m = (int)((d.m + bn - 1) / bn); p.tiles_n = (int)((d.n + kRowsX - 1) / kRowsX);
         p.idesc = f8_idesc(d, true, kRowsX, bn, a_dir, b_dir);
-        const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-        int slices = 1;
-        while (slices < 8 && tiles * slices * 2 <= 2 * g.num_sms && p.num_kb >= slices * 4) slices *= 2;
+        int slices = tile_slices;
         if (o.gemm_fp8_slices > 0) { slices = o.gemm_fp8_slices; while (slices > p.num_kb) slices /= 2; }
         p.slices = slices;
         if (tiles * slices > 0x7fffffff) { release(); *err = "too many tiles"; return ACCB_ERR_ARG; }
@@ -968,18 +1034,28 @@ int launch_gemm_fp8(const GemmFp8Launch& g0, const char** err)
     CUtensorMap ma, mb;
     if (!make_operand_map(&ma, op[0].base, d.a_type, d.m, d.k, op[0].pitch, pair ? kRowsX : bn, a_dir == 1) ||
         !make_operand_map(&mb, op[1].base, d.b_type, d.n, d.k, op[1].pitch, kRowsX, b_dir == 1)) {
+        temp_free(sums, g.stream);
         release();
         *err = "cuTensorMapEncodeTiled failed";
         return ACCB_ERR_CUDA;
     }
     cudaError_t e;
-    if (d.c_type == ACCB_F32) e = launch_c<float>(g, ma, mb, p, bn);
-    else if (d.c_type == ACCB_F16) e = launch_c<__half>(g, ma, mb, p, bn);
-    else e = launch_c<__nv_bfloat16>(g, ma, mb, p, bn);
+    if (part.d.c_type == ACCB_F32) e = launch_c<float>(part, ma, mb, p, bn);
+    else if (part.d.c_type == ACCB_F16) e = launch_c<__half>(part, ma, mb, p, bn);
+    else e = launch_c<__nv_bfloat16>(part, ma, mb, p, bn);
+    int n = 0;
+    if (e == cudaSuccess) {
+        note_launches(1);
+        n = launches + 1;
+        if (sums) {
+            const int r = launch_splitk_reduce(sums, p.slices, d, g.c, g.bias, g.stream, err, true);
+            n = r < 0 ? r : n + r;
+        }
+    }
+    temp_free(sums, g.stream);
     release();
     if (e != cudaSuccess) { *err = cudaGetErrorString(e); (void)cudaGetLastError(); return ACCB_ERR_CUDA; }
-    note_launches(1);
-    return launches + 1;
+    return n;
 }
 
 }  // namespace accb

@@ -48,7 +48,8 @@ splitk_reduce_f32_kernel(const float* __restrict__ partial, int slices, int64_t 
         float x = alpha * acc[j];
         if (beta != 0.0f) x += beta * load_as_float(d);
         if (bias) x += __ldg(bias + col0 + j);
-        if (relu) x = fmaxf(x, 0.0f);
+        if (relu == 1) x = fmaxf(x, 0.0f);
+        if (relu == 2) x = x < 0.0f ? 0.0f : x;          // a NaN stays
         store_from_float(d, x);
     }
 }
@@ -89,12 +90,12 @@ splitk_reduce_s32_kernel(const int* __restrict__ partial, int slices, int64_t m,
 }  // namespace
 
 int launch_splitk_reduce(const void* partial, int slices, const accb_gemm_desc& d, void* c, const float* bias,
-                         cudaStream_t stream, const char** err)
+                         cudaStream_t stream, const char** err, bool relu_keeps_nan)
 {
     const int64_t groups = d.m * ((d.n + 3) / 4);
     const int64_t blocks = (groups + 255) / 256;
     if (blocks > 0x7fffffff) { *err = "split-K reduction: problem too large"; return ACCB_ERR_ARG; }
-    const int relu = d.epilogue == ACCB_EPI_RELU;
+    const int relu = d.epilogue == ACCB_EPI_RELU ? (relu_keeps_nan ? 2 : 1) : 0;
     const unsigned gsz = (unsigned)blocks;
     switch (d.c_type) {
     case ACCB_F32:

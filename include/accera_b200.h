@@ -303,8 +303,8 @@ int accb_quantize_fp8(const accb_quantize_fp8_desc* desc, const void* x, void* q
  * weights' other direction contiguous, the gradient of its input; 1 and 1 is the gradient of its weights.
  *
  * Layouts: on the tensor cores each operand is contiguous along K or along its other direction; C has any strides.
- * Operands whose rows are not 16-byte aligned are copied into aligned rows first, in a stream-ordered temporary of the
- * library; nothing else is allocated.  Host or device pointers as for accb_gemm.
+ * Operands whose rows are not 16-byte aligned are copied into aligned rows first, and few-tile problems keep fp32 sums of
+ * slices of K, both in stream-ordered temporaries of the library.  Host or device pointers as for accb_gemm.
  */
 typedef struct accb_fp8_scales {
     int32_t a_block, b_block;        /* 1 or 128 */
@@ -388,8 +388,8 @@ const char* accb_version(void);
  *   "gemm.c_in"              -1 (choose) | 0 | 1      beta != 0 with warp-moved boxes: the old C is copied into the boxes ahead
  *                                                     of its use (1) or read row by row when needed (0)
  *   "gemm.verbose"           0 | 1                    print the launch plan to stderr
- *   "gemm_fp8.kernel"        0 (choose) | 1 | 2       accb_gemm_fp8: 256 x 256 tiles by CTA pairs (1), 128-column tiles with K slices (2)
- *   "gemm_fp8.slices"        0 (choose) | 1 | 2 | 4 | 8   K slices of the latter
+ *   "gemm_fp8.kernel"        0 (choose) | 1 | 2       accb_gemm_fp8: 256 x 256 tiles by CTA pairs (1), tiles of 128 columns and 16 to 64 rows (2)
+ *   "gemm_fp8.slices"        0 (choose) | 1 | 2 | 4 | 8   K slices of either
  *   "stream_kernels.pdl"     -1 (on) | 0 | 1          programmatic dependent launch of the reduce_mean, gather and range kernels
  *   "host_gemm.stage_chunks" 0 (16) | 1..256          row chunks of the staged host-pointer GEMM
  *   "reduce.rows_threads_per_output"  0 (choose) | 32 | 64 | 128 | 256   reduce_mean over contiguous segments

@@ -171,7 +171,7 @@ SHAPES = [(1, 128, 128), (1, 1, 1), (2, 130, 300), (7, 264, 512), (16, 200, 129)
 
 
 # every kernel takes every shape: which one runs is a matter of speed alone
-PATHS = {"auto": {}, "simt": {}, "pair": {"gemm_fp8.kernel": 1}, "tile": {"gemm_fp8.kernel": 2, "gemm_fp8.slices": 1},
+PATHS = {"auto": {}, "simt": {}, "pair": {"gemm_fp8.kernel": 1, "gemm_fp8.slices": 1}, "pair4": {"gemm_fp8.kernel": 1, "gemm_fp8.slices": 4}, "tile": {"gemm_fp8.kernel": 2, "gemm_fp8.slices": 1},
          "tile2": {"gemm_fp8.kernel": 2, "gemm_fp8.slices": 2}, "tile8": {"gemm_fp8.kernel": 2, "gemm_fp8.slices": 8}}
 
 
@@ -189,7 +189,7 @@ def test_gemm_equals_the_formula(path, ga, gb, m, n, k):
 @pytest.mark.parametrize("a,b", [("e4m3", "e4m3"), ("e5m2", "e4m3"), ("e4m3", "e5m2"), ("e5m2", "e5m2")])
 @pytest.mark.parametrize("c", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("layout", ["tn", "tt", "nn", "nt"])
-@pytest.mark.parametrize("path,m,n,k", [("tile", 9, 144, 272), ("tile8", 144, 272, 1040), ("pair", 272, 400, 528)])
+@pytest.mark.parametrize("path,m,n,k", [("tile", 9, 144, 272), ("tile8", 144, 272, 1040), ("pair", 272, 400, 528), ("pair4", 272, 400, 1040)])
 def test_gemm_types_and_layouts(a, b, c, layout, path, m, n, k):
     A, sa, B, sb = _operands(m, n, k, a, b, 1, 128, 3)
     sb *= 0.001                                                        # inside fp16's range
@@ -202,7 +202,7 @@ def test_gemm_types_and_layouts(a, b, c, layout, path, m, n, k):
 
 @pytest.mark.parametrize("alpha,beta,relu,use_bias", [(1.0, 1.0, False, False), (0.5, 0.0, True, True), (-2.0, 0.25, False, True), (1.0, 1.0, True, True)])
 @pytest.mark.parametrize("c", ["f32", "bf16"])
-@pytest.mark.parametrize("path", ["pair", "tile", "tile8", "simt"])
+@pytest.mark.parametrize("path", ["pair", "pair4", "tile", "tile8", "simt"])
 @pytest.mark.parametrize("m,n,k", [(1, 256, 512), (40, 203, 300), (200, 264, 768), (520, 512, 256)])
 def test_gemm_epilogue(alpha, beta, relu, use_bias, c, path, m, n, k):
     A, sa, B, sb = _operands(m, n, k, "e4m3", "e4m3", 1, 128, 4)
@@ -214,7 +214,7 @@ def test_gemm_epilogue(alpha, beta, relu, use_bias, c, path, m, n, k):
     _check(got, want, err, "epilogue")
 
 
-@pytest.mark.parametrize("path,m,n,k", [("tile", 3, 130, 256), ("tile2", 200, 300, 384), ("pair", 200, 300, 384)])
+@pytest.mark.parametrize("path,m,n,k", [("tile", 3, 130, 256), ("tile2", 200, 300, 384), ("pair", 200, 300, 384), ("pair4", 200, 300, 512)])
 def test_gemm_result_strides_leave_the_rest_alone(path, m, n, k):
     A, sa, B, sb = _operands(m, n, k, "e4m3", "e4m3", 1, 128, 5)
     want, err = _gemm_want(A, sa, B, sb, 1, 128)
