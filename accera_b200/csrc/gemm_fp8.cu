@@ -18,7 +18,8 @@
 //   tile   128 x BN tiles by single CTAs for up to 64 rows of C: columns of C (weights) on the 128 TMEM
 //          lanes, rows of C (tokens) on BN = 16 .. 64 accumulator columns, K cut into up to eight slices
 //          that a cluster multiplies side by side and adds, slice by slice, through distributed shared memory.
-// Scales reach shared memory by 4-byte cp.async (any strides), eight blocks ahead, by the warp that also issues the TMA loads.
+// Scales reach shared memory by cp.async up to sixteen blocks ahead, four blocks of a row in 16 bytes where they lie side by
+// side (4 bytes at a time the copies themselves bound the pair kernel with a scale per column).
 //
 // Every wait is bounded as in gemm_umma.cu: one that runs out is recorded, all roles leave, the host reports
 // ACCB_ERR_TIMEOUT.
@@ -50,6 +51,7 @@ struct F8Params {
     float alpha, beta;
     int relu;
     int a_shift, b_shift;                   // 0, or 7 where 128 rows of A / columns of B share a scale
+    int sa_vec, sb_vec;                     // the scales of four neighbouring blocks of a row / column lie in 16 aligned bytes
     int a_mn, b_mn;                         // operand contiguous along M / N instead of K
     int num_kb;
     uint32_t idesc;
@@ -112,6 +114,10 @@ __device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16])
 __device__ __forceinline__ void copy_scale(uint32_t dst, const float* src, bool inside)
 {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(inside ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_scales4(uint32_t dst, const float* src, bool inside)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(inside ? 16 : 0) : "memory");
 }
 // arrives on the barrier once this thread's copies so far have landed; the barrier counts one arrival a lane
 __device__ __forceinline__ void copies_arrive(uint32_t bar)
@@ -211,8 +217,59 @@ struct PairPlan {
     static_assert(kTotal <= 227 * 1024, "shared memory of a CTA");
 };
 
-// One box (32 rows of 128 bytes, this thread's row in `v`) of the tile to C, through shared memory: a row's 16-byte slots
-// are stored at slot ^ (row % 8), so neither the own-row accesses nor the ones along rows collide in banks.
+// A box between shared memory and C.  Along rows lane / 8 is one of four rows, lane % 8 a 16-byte slot; a row's slots are
+// stored at slot ^ (row % 8), so neither accesses along rows nor those of whole columns of slots collide in banks.
+template <typename TC>
+__device__ __forceinline__ void box_in(uint8_t* box, const TC* C, int64_t row0, int64_t col0, int rows, int cols, int lane, const F8Params& p)
+{
+    constexpr int V = 16 / (int)sizeof(TC);
+    const int r0 = lane >> 3, slot = lane & 7, in_slot = cols - slot * V;
+    const TC* base = C + (row0 + r0) * p.cs0 + col0 + slot * V;
+    const bool vec = p.c_mode == 2 && in_slot >= V;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + r0;
+        uint8_t* at = box + r * 128 + ((slot ^ (r & 7)) << 4);
+        const TC* src = base + (int64_t)(i * 4) * p.cs0;
+        if (r >= rows) continue;
+        if (vec) *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(src);
+        else
+            for (int e = 0; e < V && e < in_slot; ++e) reinterpret_cast<TC*>(at)[e] = src[e];
+    }
+    __syncwarp();
+}
+template <typename TC>
+__device__ __forceinline__ void box_out(const uint8_t* box, TC* C, int64_t row0, int64_t col0, int rows, int cols, int lane, const F8Params& p)
+{
+    constexpr int V = 16 / (int)sizeof(TC);
+    const int r0 = lane >> 3, slot = lane & 7, in_slot = cols - slot * V;
+    TC* base = C + (row0 + r0) * p.cs0 + col0 + slot * V;
+    const bool vec = p.c_mode == 2 && in_slot >= V;
+    __syncwarp();
+    if (p.c_mode == 2 && rows == 32 && cols == 8 * V) {
+        // a box inside the matrix, as nearly all are: all reads, then all writes
+        uint4 w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const uint4*>(box + (i * 4 + r0) * 128 + ((slot ^ ((i * 4 + r0) & 7)) << 4));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(base + (int64_t)(i * 4) * p.cs0) = w[i];
+        __syncwarp();
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + r0;
+        const uint8_t* at = box + r * 128 + ((slot ^ (r & 7)) << 4);
+        TC* dst = base + (int64_t)(i * 4) * p.cs0;
+        if (r >= rows) continue;
+        if (vec) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(at);
+        else
+            for (int e = 0; e < V && e < in_slot; ++e) dst[e] = reinterpret_cast<const TC*>(at)[e];
+    }
+    __syncwarp();
+}
+
+// One box (32 rows of 128 bytes, this thread's row in `v`) of the tile to C, through shared memory
 template <typename TC>
 __device__ __forceinline__ void store_box(float (&v)[128 / sizeof(TC)], uint8_t* box, TC* C, int64_t row0, int64_t col0, int lane, const F8Params& p)
 {
@@ -237,25 +294,10 @@ __device__ __forceinline__ void store_box(float (&v)[128 / sizeof(TC)], uint8_t*
         }
         return;
     }
-    // along rows: lane / 8 is one of four rows, lane % 8 a slot; `base` addresses that lane's 16 bytes of the first four rows
-    const int r0 = lane >> 3, slot = lane & 7;
-    TC* base = C + (row0 + r0) * p.cs0 + col0 + slot * V;
-    const int in_slot = cols - slot * V;                     // elements of the lane's slot inside the matrix
-    const bool vec = p.c_mode == 2 && in_slot >= V;
     uint8_t* own = box + lane * 128;                         // this thread's row; its slots are at s ^ (lane & 7)
     const int flip = (lane & 7) << 4;
     if (p.beta != 0.0f) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + r0;
-            uint8_t* at = box + r * 128 + ((slot ^ (r & 7)) << 4);
-            const TC* src = base + (int64_t)(i * 4) * p.cs0;
-            if (r >= rows) continue;
-            if (vec) *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(src);
-            else
-                for (int e = 0; e < V && e < in_slot; ++e) reinterpret_cast<TC*>(at)[e] = src[e];
-        }
-        __syncwarp();
+        box_in<TC>(box, C, row0, col0, rows, cols, lane, p);
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
             const uint4 w = *reinterpret_cast<const uint4*>(own + ((s << 4) ^ flip));
@@ -280,18 +322,47 @@ __device__ __forceinline__ void store_box(float (&v)[128 / sizeof(TC)], uint8_t*
         for (int e = 0; e < V; ++e) h[e] = (TC)v[s * V + e];
         *reinterpret_cast<uint4*>(own + ((s << 4) ^ flip)) = w;
     }
-    __syncwarp();
+    box_out<TC>(box, C, row0, col0, rows, cols, lane, p);
+}
+
+// The same for a thread that holds pairs of neighbouring columns of four rows, as tcgen05.ld.16x256b gives them: value(h, j, i) is
+// row 16 h + 8 (i / 2) + lane / 4, column 8 j + 2 (lane % 4) + i % 2 of the box.
+template <typename TC, typename F>
+__device__ __forceinline__ void store_box_pairs(F value, uint8_t* box, TC* C, int64_t row0, int64_t col0, int lane, const F8Params& p)
+{
+    constexpr int W = 128 / (int)sizeof(TC);
+    struct alignas(2 * sizeof(TC)) Pair { TC v[2]; };
+    const int cols = (int)(p.n - col0 < W ? p.n - col0 : W), rows = (int)(p.m - row0 < 32 ? p.m - row0 : 32);
+    const bool boxed = p.c_mode != 0;
+    if (boxed && p.beta != 0.0f) box_in<TC>(box, C, row0, col0, rows, cols, lane, p);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int r = i * 4 + r0;
-        const uint8_t* at = box + r * 128 + ((slot ^ (r & 7)) << 4);
-        TC* dst = base + (int64_t)(i * 4) * p.cs0;
-        if (r >= rows) continue;
-        if (vec) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(at);
-        else
-            for (int e = 0; e < V && e < in_slot; ++e) dst[e] = reinterpret_cast<const TC*>(at)[e];
+    for (int j = 0; j < W / 8; ++j) {
+        const int col = 8 * j + 2 * (lane & 3);
+        float bias[2] = { 0.0f, 0.0f };
+        if (p.bias) {
+            if (col < cols) bias[0] = __ldg(p.bias + col0 + col);
+            if (col + 1 < cols) bias[1] = __ldg(p.bias + col0 + col + 1);
+        }
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const int row = 8 * h + (lane >> 2);
+            const float lo = value(h >> 1, j, 2 * (h & 1)), hi = value(h >> 1, j, 2 * (h & 1) + 1);
+            if (boxed) {
+                const int byte = col * (int)sizeof(TC);
+                Pair* at = reinterpret_cast<Pair*>(box + row * 128 + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15));
+                Pair y = {};
+                if (p.beta != 0.0f) y = *at;
+                y.v[0] = (TC)finish(lo, (float)y.v[0], bias[0], p);
+                y.v[1] = (TC)finish(hi, (float)y.v[1], bias[1], p);
+                *at = y;
+            } else if (row < rows) {
+                TC* d = C + (row0 + row) * p.cs0 + (col0 + col) * p.cs1;
+                if (col < cols) d[0] = (TC)finish(lo, p.beta != 0.0f ? (float)d[0] : 0.0f, bias[0], p);
+                if (col + 1 < cols) d[p.cs1] = (TC)finish(hi, p.beta != 0.0f ? (float)d[p.cs1] : 0.0f, bias[1], p);
+            }
+        }
     }
-    __syncwarp();
+    if (boxed) box_out<TC>(box, C, row0, col0, rows, cols, lane, p);
 }
 
 // work item -> tile and range of blocks of K
@@ -314,20 +385,39 @@ __device__ __forceinline__ void pair_item(int t, const F8Params& p, int& tm, int
     tn = in / rows;
 }
 
-// 32 columns of a block's product, times the product of the scales, to the sums: one scale for all, or one for each column
+// 32 columns of a block's product, times one scale, to the sums
 __device__ __forceinline__ void add_scaled(float* acc, const uint32_t (&x)[32], float f)
 {
 #pragma unroll
     for (int j = 0; j < 32; ++j) acc[j] = fmaf(__uint_as_float(x[j]), f, acc[j]);
 }
-__device__ __forceinline__ void add_scaled(float* acc, const uint32_t (&x)[32], float f, const float4 (&w)[8])
+// 32 columns of 32 lanes as two 16x256b loads: register 16 h + 4 j + i of lane l is row 16 h + 8 (i / 2) + l / 4, column
+// 8 j + 2 (l % 4) + i % 2
+__device__ __forceinline__ void tmem_ld_pairs(uint32_t taddr, uint32_t (&r)[32])
 {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        acc[4 * j] = fmaf(__uint_as_float(x[4 * j]), f * w[j].x, acc[4 * j]);
-        acc[4 * j + 1] = fmaf(__uint_as_float(x[4 * j + 1]), f * w[j].y, acc[4 * j + 1]);
-        acc[4 * j + 2] = fmaf(__uint_as_float(x[4 * j + 2]), f * w[j].z, acc[4 * j + 2]);
-        acc[4 * j + 3] = fmaf(__uint_as_float(x[4 * j + 3]), f * w[j].w, acc[4 * j + 3]);
+    for (int h = 0; h < 2; ++h)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+            : "=r"(r[16 * h]), "=r"(r[16 * h + 1]), "=r"(r[16 * h + 2]), "=r"(r[16 * h + 3]), "=r"(r[16 * h + 4]), "=r"(r[16 * h + 5]),
+              "=r"(r[16 * h + 6]), "=r"(r[16 * h + 7]), "=r"(r[16 * h + 8]), "=r"(r[16 * h + 9]), "=r"(r[16 * h + 10]), "=r"(r[16 * h + 11]),
+              "=r"(r[16 * h + 12]), "=r"(r[16 * h + 13]), "=r"(r[16 * h + 14]), "=r"(r[16 * h + 15])
+            : "r"(taddr + ((uint32_t)(16 * h) << 16))
+            : "memory");
+}
+// the same columns, times a scale for each of this thread's four rows and each of its two columns in eight (at col_scale,
+// four floats a column)
+__device__ __forceinline__ void add_scaled_pairs(float* acc, const uint32_t (&x)[32], const float (&f)[4], const float* col_scale)
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 w = make_float2(col_scale[32 * j], col_scale[32 * j + 4]);
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const int i = 16 * (h >> 1) + 4 * j + 2 * (h & 1);
+            acc[i] = fmaf(__uint_as_float(x[i]), f[h] * w.x, acc[i]);
+            acc[i + 1] = fmaf(__uint_as_float(x[i + 1]), f[h] * w.y, acc[i + 1]);
+        }
     }
 }
 
@@ -423,21 +513,21 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 ok = __all_sync(0xffffffffu, mbar_wait(scale_empty_bar(r), rph ^ 1u, wctx, SITE_PRODUCER_EMPTY, kb0));
                 if (!ok) break;
                 const int blocks = min(Plan::kGroup, kb_end - kb0);
-                for (int j = 0; j < blocks; ++j) {
-                    const uint32_t sc = smem_base + Plan::kScales + (r * Plan::kGroup + j) * Plan::kScaleBytes;
-                    const float* sa = p.sa + (kb0 + j) * p.sa_kb;
-                    const float* sb = p.sb + (kb0 + j) * p.sb_kb;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int64_t row = row_a + i * 32;
-                        copy_scale(sc + (i * 32 + lane) * 4, sa + (row < p.m ? (row >> p.a_shift) * p.sa_row : 0), row < p.m);
+                const uint32_t slot = smem_base + Plan::kScales + r * Plan::kGroup * Plan::kScaleBytes;
+                auto copy = [&](const float* base, int64_t first, int64_t count, int64_t step, int shift, int64_t s_row, int64_t s_kb, int loads, int at, int vec) {
+                    for (int i = 0; i < loads; ++i) {
+                        const int64_t row = first + i * step;
+                        const bool inside = row < count;
+                        const float* src = base + (inside ? (row >> shift) * s_row : 0) + kb0 * s_kb;
+                        const uint32_t dst = slot + (at + i * 32 + lane) * 16;
+                        if (vec) copy_scales4(dst, src, inside);
+                        else
+                            for (int j = 0; j < blocks; ++j) copy_scale(dst + 4 * j, src + j * s_kb, inside);
                     }
-#pragma unroll
-                    for (int i = 0; i < (COLS ? 8 : 1); ++i) {
-                        const int64_t col = col_b + i * 32;
-                        if (COLS || lane < 2) copy_scale(sc + (kRowsX + i * 32 + lane) * 4, sb + (col < p.n ? (col >> p.b_shift) * p.sb_col : 0), col < p.n);
-                    }
-                }
+                };
+                const bool whole = blocks == Plan::kGroup && kb0 % Plan::kGroup == 0;
+                copy(p.sa, row_a, p.m, 32, p.a_shift, p.sa_row, p.sa_kb, 4, 0, p.sa_vec && whole);
+                if (COLS || lane < 2) copy(p.sb, col_b, p.n, 32, p.b_shift, p.sb_col, p.sb_kb, COLS ? 8 : 1, kRowsX, p.sb_vec && whole);
                 copies_arrive(scale_full_bar(r));
                 if (++r == Plan::kSlots) { r = 0; rph ^= 1u; }
             }
@@ -503,51 +593,48 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    tmem_ld32(taddr, x0);
+                    if constexpr (COLS) tmem_ld_pairs(taddr, x0);
+                    else tmem_ld32(taddr, x0);
                 }
                 if (++s == S) { s = 0; ph ^= 1u; }
-                const float* sc = scales + (r * Plan::kGroup + in_group) * (Plan::kScaleBytes / 4);
-                const float* col_scale = sc + kRowsX + (COLS ? half * 128 : half);
+                // a slot holds the scales of a row, or column, of four blocks side by side
+                const float* sc = scales + r * Plan::kGroup * (Plan::kScaleBytes / 4) + in_group;
+                const float* col_scale = sc + 4 * (kRowsX + (COLS ? half * 128 : half));
+                // A column's scale for each thread that holds the column costs shared memory as much bandwidth as the sums cost
+                // TMEM, 1024 cycles a block with a row a thread.  With pairs of columns of four rows a thread it is a quarter.
+                float f[COLS ? 4 : 1];
                 if constexpr (COLS) {
-                    // the columns' scales need the registers of a second load: they are read while the one load is on its way
-                    const float f = sc[q * 32 + lane];
+                    col_scale += 8 * (lane & 3);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float4 w[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) w[j] = *reinterpret_cast<const float4*>(col_scale + 32 * c + 4 * j);
-                        tmem_wait_ld(x0);
-                        if (c == 3) {
-                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive_pair(tmem_empty_bar(buf) & kPeerMask);
-                        }
-                        add_scaled(acc + 32 * c, x0, f, w);
-                        if (c < 3) tmem_ld32(taddr + 32 * (c + 1), x0);
-                    }
+                    for (int i = 0; i < 4; ++i) f[i] = sc[4 * (q * 32 + (lane >> 2) + 8 * i)];
                 } else {
-                    const float f = sc[q * 32 + lane] * col_scale[0];
-                    tmem_wait_ld(x0);
-                    tmem_ld32(taddr + 32, x1);
-                    add_scaled(acc, x0, f);
-                    tmem_wait_ld(x1);
-                    tmem_ld32(taddr + 64, x0);
-                    add_scaled(acc + 32, x1, f);
-                    tmem_wait_ld(x0);
-                    tmem_ld32(taddr + 96, x1);
-                    const bool next = kb + 1 < num_kb && mbar_test(done_bar(s), ph);
-                    add_scaled(acc + 64, x0, f);
-                    tmem_wait_ld(x1);
-                    // this warp has read the buffer: the MMA issuer of the pair may overwrite it
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    loading = __all_sync(0xffffffffu, next);
-                    if (lane == 0) mbar_arrive_pair(tmem_empty_bar(buf) & kPeerMask);
-                    if (loading) {
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        tmem_ld32(taddr0 + (uint32_t)((buf ^ 1) * Plan::kBN), x0);
-                    }
-                    add_scaled(acc + 96, x1, f);
+                    f[0] = sc[4 * (q * 32 + lane)] * col_scale[0];
                 }
+                auto load = [&](uint32_t at, uint32_t (&x)[32]) { if constexpr (COLS) tmem_ld_pairs(at, x); else tmem_ld32(at, x); };
+                auto add = [&](int c, const uint32_t (&x)[32]) {
+                    if constexpr (COLS) add_scaled_pairs(acc + 32 * c, x, f, col_scale + 128 * c);
+                    else add_scaled(acc + 32 * c, x, f[0]);
+                };
+                tmem_wait_ld(x0);
+                load(taddr + 32, x1);
+                add(0, x0);
+                tmem_wait_ld(x1);
+                load(taddr + 64, x0);
+                add(1, x1);
+                tmem_wait_ld(x0);
+                load(taddr + 96, x1);
+                const bool next = kb + 1 < num_kb && mbar_test(done_bar(s), ph);
+                add(2, x0);
+                tmem_wait_ld(x1);
+                // this warp has read the buffer: the MMA issuer of the pair may overwrite it
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                loading = __all_sync(0xffffffffu, next);
+                if (lane == 0) mbar_arrive_pair(tmem_empty_bar(buf) & kPeerMask);
+                if (loading) {
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    load(taddr0 + (uint32_t)((buf ^ 1) * Plan::kBN), x0);
+                }
+                add(3, x1);
                 if (in_group == Plan::kGroup - 1 || kb == num_kb - 1) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(scale_empty_bar(r));
@@ -559,10 +646,16 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             constexpr int W = 128 / (int)sizeof(TC);
 #pragma unroll
             for (int b = 0; b < 128 / W; ++b) {
-                float v[W];
+                if (row0 >= p.m || col0 + b * W >= p.n) continue;
+                TC* dst = SPLIT ? C + slice * p.slice_stride : C;
+                if constexpr (COLS) {
+                    store_box_pairs<TC>([&](int h, int j, int i) { return acc[b * W + 32 * (j / 4) + 16 * h + 4 * (j % 4) + i]; }, box, dst, row0, col0 + b * W, lane, p);
+                } else {
+                    float v[W];
 #pragma unroll
-                for (int j = 0; j < W; ++j) v[j] = acc[b * W + j];
-                if (row0 < p.m && col0 + b * W < p.n) store_box<TC>(v, box, SPLIT ? C + slice * p.slice_stride : C, row0, col0 + b * W, lane, p);
+                    for (int j = 0; j < W; ++j) v[j] = acc[b * W + j];
+                    store_box<TC>(v, box, dst, row0, col0 + b * W, lane, p);
+                }
             }
         }
         if (!ok && lane == 0) record_give_up();
@@ -969,6 +1062,8 @@ int launch_gemm_fp8(const GemmFp8Launch& g0, const char** err)
     p.a_shift = g.s.a_block == 1 ? 0 : 7; p.b_shift = g.s.b_block == 1 ? 0 : 7;
     p.alpha = d.alpha; p.beta = d.beta; p.relu = d.epilogue == ACCB_EPI_RELU;
     p.a_mn = a_dir; p.b_mn = b_dir;
+    p.sa_vec = p.sa_kb == 1 && p.sa_row % 4 == 0 && (reinterpret_cast<uintptr_t>(p.sa) & 15) == 0;
+    p.sb_vec = p.sb_kb == 1 && p.sb_col % 4 == 0 && (reinterpret_cast<uintptr_t>(p.sb) & 15) == 0;
     p.num_kb = (int)((d.k + kSlabBytes - 1) / kSlabBytes);
     p.status = g.status; p.launch_id = g.launch_id;
     const Options& o = options();
