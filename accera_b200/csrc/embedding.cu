@@ -276,7 +276,7 @@ __device__ __forceinline__ void clear_rows(TT* table, const void* ids, int part,
     __syncthreads();
     // as many threads side by side as a row has vectors: the CTA writes one stretch of memory after the other
     constexpr int V = 16 / (int)sizeof(TT);
-    const int width = c.vec ? c.dim / V : c.dim;
+    const int width = c.beta == 0.0f ? (c.dim + V - 1) / V : c.dim;
     int per_row = 32;
     while (per_row < 256 && per_row < width) per_row *= 2;
     const int sub = threadIdx.x / per_row, x = threadIdx.x % per_row;
@@ -289,7 +289,12 @@ __device__ __forceinline__ void clear_rows(TT* table, const void* ids, int part,
         } else if (c.vec) {
             for (int v = x; v < width; v += per_row) reinterpret_cast<uint4*>(row)[v] = make_uint4(0u, 0u, 0u, 0u);
         } else {
-            for (int i = x; i < c.dim; i += per_row) row[i] = (TT)0.0f;
+            // a row that starts or ends within a vector: its whole vectors, and the elements before and after them
+            const int head = min(c.dim, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(TT)), vecs = (c.dim - head) / V;
+            for (int v = x; v < vecs; v += per_row) reinterpret_cast<uint4*>(row + head)[v] = make_uint4(0u, 0u, 0u, 0u);
+            const int tail = head + vecs * V;
+            if (x < head) row[x] = (TT)0.0f;
+            if (tail + x < c.dim && x < V) row[tail + x] = (TT)0.0f;
         }
     }
 }
@@ -552,47 +557,61 @@ few_tokens_kernel(const TR* __restrict__ rows, const void* __restrict__ ids, TT*
             n += count[r][w];
         }
     __syncthreads();
-    auto add_rows = [&](int begin, int step, int col, float (&acc)[E]) {
-        for (int j0 = begin; j0 < n; j0 += step * kFewUnroll) {
-            Vec<TR, E> x[kFewUnroll];
-#pragma unroll
-            for (int u = 0; u < kFewUnroll; ++u)
-                if (j0 + u * step < n) x[u] = *reinterpret_cast<const Vec<TR, E>*>(rows + (int64_t)list[j0 + u * step] * p.rows_stride + col);
-#pragma unroll
-            for (int u = 0; u < kFewUnroll; ++u)
-                if (j0 + u * step < n) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) acc[e] += (float)x[u].v[e];
-                }
-        }
-    };
     if (n <= kFewSplit) {
         const int col = (slab * kFewThreads + threadIdx.x) * E;
         if (col >= p.dim) return;
         float acc[E] = {};
-        add_rows(0, 1, col, acc);
+        for (int j0 = 0; j0 < n; j0 += kFewUnroll) {
+            Vec<TR, E> x[kFewUnroll];
+#pragma unroll
+            for (int u = 0; u < kFewUnroll; ++u)
+                if (j0 + u < n) x[u] = *reinterpret_cast<const Vec<TR, E>*>(rows + (int64_t)list[j0 + u] * p.rows_stride + col);
+#pragma unroll
+            for (int u = 0; u < kFewUnroll; ++u)
+                if (j0 + u < n) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] += (float)x[u].v[e];
+                }
+        }
         write_sum<TT, E>(table, word, p.table_stride, col, acc, p.scale, p.beta);
         return;
     }
-    constexpr int kCols = kFewThreads / kFewLanes;
+    // kAtOnce of the slab's eighths together: their loads of a row do not wait for one another
+    constexpr int kCols = kFewThreads / kFewLanes, kAtOnce = E == 1 ? 8 : 2;
     const int x = threadIdx.x % kCols, y = threadIdx.x / kCols;
-    for (int v0 = 0; v0 < kFewThreads; v0 += kCols) {
-        const int col = (slab * kFewThreads + v0 + x) * E;
-        float acc[E] = {};
-        if (col < p.dim) add_rows(y, kFewLanes, col, acc);
+    for (int v0 = 0; v0 < kFewThreads; v0 += kCols * kAtOnce) {
+        float acc[kAtOnce][E] = {};
+        const int col0 = (slab * kFewThreads + v0 + x) * E;
+#pragma unroll 2
+        for (int j = y; j < n; j += kFewLanes) {
+            const TR* row = rows + (int64_t)list[j] * p.rows_stride;
+            Vec<TR, E> v[kAtOnce];
 #pragma unroll
-        for (int e = 0; e < E; ++e) part[y][x][e] = acc[e];
-        __syncthreads();
-        if (y == 0 && col < p.dim) {
+            for (int a = 0; a < kAtOnce; ++a)
+                if (col0 + a * kCols * E < p.dim) v[a] = *reinterpret_cast<const Vec<TR, E>*>(row + col0 + a * kCols * E);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                acc[e] = 0.0f;
+            for (int a = 0; a < kAtOnce; ++a)
+                if (col0 + a * kCols * E < p.dim) {
 #pragma unroll
-                for (int l = 0; l < kFewLanes; ++l) acc[e] += part[l][x][e];
-            }
-            write_sum<TT, E>(table, word, p.table_stride, col, acc, p.scale, p.beta);
+                    for (int e = 0; e < E; ++e) acc[a][e] += (float)v[a].v[e];
+                }
         }
-        __syncthreads();
+#pragma unroll
+        for (int a = 0; a < kAtOnce; ++a) {
+            const int col = col0 + a * kCols * E;
+#pragma unroll
+            for (int e = 0; e < E; ++e) part[y][x][e] = acc[a][e];
+            __syncthreads();
+            if (y == 0 && col < p.dim) {
+                float sum[E] = {};
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+#pragma unroll
+                    for (int l = 0; l < kFewLanes; ++l) sum[e] += part[l][x][e];
+                write_sum<TT, E>(table, word, p.table_stride, col, sum, p.scale, p.beta);
+            }
+            __syncthreads();
+        }
     }
 }
 
