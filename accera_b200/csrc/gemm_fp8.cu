@@ -863,29 +863,12 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Plan::kTmemCols) : "memory");
     }
 
-    // All loads and MMAs of this CTA are done: the operand ring may hold the slice's sums, [BN][128] fp32.
-    const int cols = (int)(p.m - col0 < BN ? p.m - col0 : BN), at = (warp & 3) * 32 + lane;
-    // element (token c of the tile, weight r of the tile)
-    auto put = [&](int c, int r, float v) {
-        const int64_t n_index = (int64_t)row0 + r;
-        if (n_index >= p.n) return;
-        TC* d = C + (col0 + c) * p.cs0 + n_index * p.cs1;
-        *d = (TC)finish(v, p.beta != 0.0f ? (float)*d : 0.0f, p.bias ? __ldg(p.bias + n_index) : 0.0f, p);
-    };
-    if (p.slices == 1) {
-        if (warp >= 2) {
-#pragma unroll
-            for (int c = 0; c < BN; c += 2) {
-                float lo, hi;
-                unpack2(acc[c / 2], lo, hi);
-                if (c < cols) put(c, at, lo);
-                if (c + 1 < cols) put(c + 1, at, hi);
-            }
-        }
-        return;
-    }
+    // All loads and MMAs of this CTA are done: the operand ring holds the slice's sums, [BN][128] fp32, which leave with four
+    // weights a lane, so that a token's 128 results are one or two instructions of a warp.
+    const int cols = (int)(p.m - col0 < BN ? p.m - col0 : BN);
     float* sums = reinterpret_cast<float*>(smem_gen);
     if (warp >= 2) {
+        const int at = (warp & 3) * 32 + lane;
 #pragma unroll
         for (int c = 0; c < BN; c += 2) {
             float lo, hi;
@@ -894,33 +877,49 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             sums[(c + 1) * kRowsX + at] = hi;
         }
     }
-    cluster_sync_all();
-    if (warp >= 2) {
-        // This CTA's share of the columns: every slices-th, one a warp at a time, four weights a lane; the slices' sums are
-        // added in their order along K.  Reads from other CTAs take long, so those of two columns are issued together.
+    const int64_t n0 = (int64_t)row0 + lane * 4;
+    float bias[4] = {};
+    if (p.bias) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (n0 + e < p.n) bias[e] = __ldg(p.bias + n0 + e);
+    }
+    if (p.slices > 1) cluster_sync_all(); else __syncthreads();
+    if (warp >= 2 && n0 < p.n) {
+        // This CTA's share of the columns: every slices-th, one a warp at a time; the slices' sums are added in their order
+        // along K.  Reads from other CTAs take long, so those of two columns are issued together.
+        struct alignas(4 * sizeof(TC)) Four { TC v[4]; };
+        const bool vec = p.cs1 == 1 && n0 + 4 <= p.n && p.cs0 % 4 == 0 && reinterpret_cast<uintptr_t>(C) % sizeof(Four) == 0;
         const int step = p.slices * 4;
         for (int c = slice + p.slices * (warp - 2); c < cols; c += 2 * step) {
-            float4 v[2] = {};
+            float v[2][4] = {};
             const bool two = c + step < cols;
+            const uint32_t mine = smem_base + (uint32_t)(c * kRowsX + lane * 4) * 4, second = two ? (uint32_t)(step * kRowsX) * 4 : 0u;
 #pragma unroll 4
             for (int z = 0; z < p.slices; ++z) {
-                const uint32_t other = map_to_rank(smem_base + (uint32_t)(c * kRowsX + lane * 4) * 4, (uint32_t)z);
-                const float4 a = load_cluster4(other);
-                const float4 b = load_cluster4(two ? other + (uint32_t)(step * kRowsX) * 4 : other);
-                v[0].x += a.x; v[0].y += a.y; v[0].z += a.z; v[0].w += a.w;
-                v[1].x += b.x; v[1].y += b.y; v[1].z += b.z; v[1].w += b.w;
+                const uint32_t from = p.slices > 1 ? map_to_rank(mine, (uint32_t)z) : mine;
+                const float4 a = load_cluster4(from), b = load_cluster4(from + second);
+                v[0][0] += a.x; v[0][1] += a.y; v[0][2] += a.z; v[0][3] += a.w;
+                v[1][0] += b.x; v[1][1] += b.y; v[1][2] += b.z; v[1][3] += b.w;
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (h == 1 && !two) break;
-                put(c + h * step, lane * 4, v[h].x);
-                put(c + h * step, lane * 4 + 1, v[h].y);
-                put(c + h * step, lane * 4 + 2, v[h].z);
-                put(c + h * step, lane * 4 + 3, v[h].w);
+                TC* d = C + (col0 + c + h * step) * p.cs0 + n0 * p.cs1;
+                if (vec) {
+                    Four y = {};
+                    if (p.beta != 0.0f) y = *reinterpret_cast<const Four*>(d);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y.v[e] = (TC)finish(v[h][e], (float)y.v[e], bias[e], p);
+                    *reinterpret_cast<Four*>(d) = y;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (n0 + e < p.n) d[e * p.cs1] = (TC)finish(v[h][e], p.beta != 0.0f ? (float)d[e * p.cs1] : 0.0f, bias[e], p);
+                }
             }
         }
     }
-    cluster_sync_all();                                                  // nobody leaves while its sums are being read
+    if (p.slices > 1) cluster_sync_all();                                // nobody leaves while its sums are being read
 }
 
 // ---------------------------------------------------------------------------------
