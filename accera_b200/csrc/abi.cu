@@ -875,7 +875,7 @@ static int embedding_entry(const char* fn, bool grad, const accb_embedding_desc*
     const accb_embedding_desc& d = *desc;
     if (d.tokens < 0 || d.vocab < 0 || d.dim < 0) return fail(ACCB_ERR_ARG, who + "negative dimension");
     const int64_t lim = ((int64_t)1 << 31) - 1;
-    if (d.tokens >= lim || d.vocab >= lim || d.dim >= lim) return fail(ACCB_ERR_ARG, who + "dimension too large");
+    if (d.tokens > (int64_t)1 << 30 || d.vocab >= lim || d.dim >= lim) return fail(ACCB_ERR_ARG, who + "dimension too large");
     if (d.dim > (int64_t)1 << 20) return fail(ACCB_ERR_ARG, who + "dim is at most 2^20");
     if (!is_float_type(d.table_type) || !is_float_type(d.rows_type)) return fail(ACCB_ERR_ARG, who + "table and rows are fp32, fp16 or bf16");
     if (d.id_bytes != 4 && d.id_bytes != 8) return fail(ACCB_ERR_ARG, who + "id_bytes must be 4 or 8");

@@ -62,6 +62,7 @@ struct F8Params {
     int* status;
     int launch_id;
     unsigned long long wait_ns;
+    int drop_commit;                        // self-test of the time-out path: the commit of the last block's MMAs is left out
 };
 
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi)
@@ -556,7 +557,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t stage = (uint64_t)(s * (Plan::kStageBytes >> 4));
                 mma_block<true>(tmem_base + (uint32_t)((g & 1) * Plan::kBN), a0 + stage, b0 + stage, p.idesc, a_step, b_step, elected);
-                if (elected) umma_commit<true>(done_bar(s));
+                if (elected && !(p.drop_commit && g == blocks - 1)) umma_commit<true>(done_bar(s));
                 __syncwarp();
                 if (++s == S) { s = 0; ph ^= 1u; }
             }
@@ -807,7 +808,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                     const uint32_t sw = smem_base + s * Plan::kStageBytes;
                     issue_stage<KIND_F8F6F4, false, W_MN, T_MN>(tmem_base + (uint32_t)(b * BN), sw, sw + kRowsX * kSlabBytes, p.idesc, true);
                     umma_commit<false>(empty_bar(s));
-                    umma_commit<false>(tmem_full_bar(b));
+                    if (!(p.drop_commit && kb == kb_end - 1)) umma_commit<false>(tmem_full_bar(b));
                     if (++s == S) { s = 0; ph ^= 1u; }
                     if (++b == NB) { b = 0; bph ^= 1u; }
                 }
@@ -1066,6 +1067,7 @@ int launch_gemm_fp8(const GemmFp8Launch& g0, const char** err)
     p.num_kb = (int)((d.k + kSlabBytes - 1) / kSlabBytes);
     p.status = g.status; p.launch_id = g.launch_id;
     const Options& o = options();
+    p.drop_commit = o.gemm_test_drop_commit;
     p.wait_ns = o.gemm_wait_limit_us > 0 ? (unsigned long long)o.gemm_wait_limit_us * 1000ull : 1000000000ull;
 
     // Which kernel, and how many slices of K, by estimated microseconds, fitted to measured launches (graph replays).

@@ -241,9 +241,10 @@ int accb_gather_rank2_dims(int64_t d0, int64_t d1, int64_t i0, int64_t i1, int32
  *
  * An id outside [0, vocab) is not dereferenced: its row is zero-filled (lookup) or left out (gradient) and
  * ACCB_ERR_INDEX is reported, from this call for host pointers and from the next accb_synchronize() for device
- * pointers.  Neither array may overlap the other.  A device-pointer accb_embedding_grad takes its workspace (16 bytes a
- * token and some partial sums) from a stream-ordered pool of the library, so calls on several streams do not share it.
- * tokens and vocab are below 2^31 - 1, dim is at most 2^20.
+ * pointers.  Neither array may overlap the other.  A device-pointer accb_embedding_grad of more than
+ * 1024 tokens takes its workspace (16 bytes a token and some partial sums) from a stream-ordered pool of the library, so calls on
+ * several streams, and captured graphs, do not share it.
+ * tokens is at most 2^30, vocab below 2^31 - 1, dim at most 2^20.
  */
 typedef struct accb_embedding_desc {
     int64_t tokens, vocab, dim;
@@ -298,8 +299,8 @@ int accb_quantize_fp8(const accb_quantize_fp8_desc* desc, const void* x, void* q
  * and the sum over blocks are accumulated in fp32; the product of a block's two scales is rounded to fp32 first.
  *
  * a_scales is ceil(M / a_block) x ceil(K / 128), b_scales ceil(K / 128) x ceil(N / b_block), a_block and b_block each
- * 1 (a scale per row of A / column of B) or 128, any positive strides; any fp32 value may be a scale.  A product whose
- * block sum is infinite or NaN stays so.  Activations (a_block = 1) times weights (b_block = 128) is the forward product and, with the
+ * 1 (a scale per row of A / column of B) or 128, any positive strides; any fp32 value may be a scale.  Infinities
+ * and NaN of a block stay with their row or column, also through the ReLU.  Activations (a_block = 1) times weights (b_block = 128) is the forward product and, with the
  * weights' other direction contiguous, the gradient of its input; 1 and 1 is the gradient of its weights.
  *
  * Layouts: on the tensor cores each operand is contiguous along K or along its other direction; C has any strides.
@@ -378,7 +379,7 @@ const char* accb_version(void);
  *   "gemm.copy_ctas"         -1 (choose) | 0..128     accb_gemm_replicated: CTAs set aside to forward finished tiles to the
  *                                                     replicas (0: the computing CTAs store to every replica themselves)
  *   "gemm.wait_limit_us"     0 (one second) | us      limit of every bounded device-side wait
- *   "gemm.test_drop_commit"  0 | 1                    self-test: each CTA's last accumulator is never signalled complete,
+ *   "gemm.test_drop_commit"  0 | 1                    self-test (accb_gemm, accb_gemm_fp8): each CTA's last accumulator is never signalled complete,
  *                                                     so the epilogue's bounded wait runs out and the launch reports
  *                                                     ACCB_ERR_TIMEOUT (no fault, no trap; the context stays usable)
  *   "gemm.pdl"               -1 (on) | 0 | 1          programmatic dependent launch: the next GEMM of a stream is scheduled

@@ -54,7 +54,7 @@ def test_packed_descriptors_have_the_structures_layout():
 def test_embedding_descriptor():
     p = ctypes.c_void_p(64)
     good = dict(tokens=3, vocab=9, dim=8, table_type=rt.F32, rows_type=rt.BF16, id_bytes=8, reserved=0, table_stride=8, rows_stride=8, padding_id=-1, scale=1.0, beta=0.0)
-    for change, text in [(dict(tokens=-1), "negative"), (dict(vocab=1 << 31), "too large"), (dict(dim=(1 << 20) + 1), "2^20"), (dict(table_type=rt.S32), "fp32, fp16 or bf16"),
+    for change, text in [(dict(tokens=-1), "negative"), (dict(vocab=1 << 31), "too large"), (dict(tokens=(1 << 30) + 1), "too large"), (dict(dim=(1 << 20) + 1), "2^20"), (dict(table_type=rt.S32), "fp32, fp16 or bf16"),
                          (dict(rows_type=rt.E4M3), "fp32, fp16 or bf16"), (dict(id_bytes=2), "id_bytes"), (dict(reserved=1), "reserved"), (dict(table_stride=7), "at least dim"),
                          (dict(rows_stride=0), "at least dim")]:
         d = rt.EmbeddingDesc(**{**good, **change})
@@ -125,6 +125,14 @@ def test_gemm_arguments():
     assert _c("accb_gemm_fp8", ctypes.byref(d), ctypes.byref(s), None, p, p, p, p, None)[0] == rt.ERR_ARG
     d.m = 0
     assert _c("accb_gemm_fp8", ctypes.byref(d), ctypes.byref(s), None, None, None, None, None, None)[0] == 0
+
+
+def test_options_of_the_8_bit_gemm():
+    for name, value in (("gemm_fp8.kernel", 3), ("gemm_fp8.slices", 3), ("gemm_fp8.slices", -1)):
+        with pytest.raises(rt.AccbError, match=name):
+            rt.set_option(name, value)
+    with rt.options(**{"gemm_fp8.kernel": 2, "gemm_fp8.slices": 8}):
+        pass
 
 
 def test_valid_host_calls_need_a_gpu():

@@ -308,6 +308,44 @@ def test_gemm_streams_graphs_and_equal_bits(m, n, k):
     assert torch.equal(got[0], want) and torch.equal(got[1], want)
 
 
+@pytest.mark.parametrize("path", ["pair", "tile", "tile2"])
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(path):
+    A, sa, B, sb = _operands(150, 300, 512, "e4m3", "e4m3", 1, 1, 10)
+    want, err = _gemm_want(A, sa, B, sb, 1, 1)
+    rt.synchronize()
+    with rt.options(**PATHS[path], **{"gemm.test_drop_commit": 1, "gemm.wait_limit_us": 20000}):
+        C = torch.zeros(150, 300, device="cuda")
+        rt.gemm_fp8(A.cuda(), B.cuda().t(), C, sa.cuda(), sb.cuda().t(), beta=0.0)
+        with pytest.raises(rt.AccbError) as e:
+            rt.synchronize()
+        assert e.value.code == rt.ERR_TIMEOUT and "epilogue waiting" in str(e.value)
+    with rt.options(**PATHS[path]):
+        _check(_run(A, sa, B, sb, 1, 1, "f32"), want, err, path)
+
+
+@pytest.mark.parametrize("max_ctas", [1, 2, 7, 1000])
+def test_gemm_on_a_bounded_grid(max_ctas):
+    A, sa, B, sb = _operands(700, 600, 640, "e4m3", "e4m3", 1, 128, 11)
+    want, err = _gemm_want(A, sa, B, sb, 1, 128)
+    _check(_run(A, sa, B, sb, 1, 128, "bf16", max_ctas=max_ctas), want, err, max_ctas)
+
+
+def test_scales_in_any_layout():
+    # four blocks' scales of a row side by side and aligned, the same unaligned, block-major, and every second value
+    m, n, k = 300, 520, 2048
+    A, sa, B, sb = _operands(m, n, k, "e4m3", "e4m3", 1, 1, 12)
+    want, err = _gemm_want(A, sa, B, sb, 1, 1)
+    Ad, Bd = A.cuda(), B.cuda().t()
+    for make in (lambda s: s.cuda(), lambda s: torch.zeros(s.shape[0], s.shape[1] + 3, device="cuda")[:, 1:17].copy_(s), lambda s: s.t().contiguous().cuda().t(),
+                 lambda s: torch.zeros(s.shape[0], 2 * s.shape[1], device="cuda")[:, ::2].copy_(s)):
+        for path in ("pair", "pair4", "tile", "simt"):
+            C = torch.zeros(m, n, device="cuda")
+            with rt.options(**PATHS[path]):
+                rt.gemm_fp8(Ad, Bd, C, make(sa), make(sb).t(), beta=0.0, compute="simt" if path == "simt" else "auto")
+            rt.synchronize()
+            _check(C.cpu(), want, err, (path, make(sa).stride()))
+
+
 def test_host_arrays():
     rng = np.random.default_rng(2)
     x = rng.standard_normal((33, 300), dtype=np.float32)
