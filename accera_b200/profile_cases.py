@@ -8,6 +8,9 @@
     python -m accera_b200.profile_cases gemm_f16 | gemm_s8 | gemm_tf32 [--m --n --k]      (row-major A, column-major B)
     python -m accera_b200.profile_cases reduce_cols [--rows 4096 --cols 8192]              (mean over the first axis)
     python -m accera_b200.profile_cases gather_elem [--table-rows 4096 --cols 32000 --indices 16384]   (gather along axis 1)
+    python -m accera_b200.profile_cases gemm_fp8 [--m --n --k] [--column-scales]           (e4m3, one scale per 128 along K)
+    python -m accera_b200.profile_cases quantize_fp8 [--rows 8192 --cols 8192] [--across]
+    python -m accera_b200.profile_cases embedding | embedding_grad [--table-rows 32000 --cols 4096 --indices 16384]
 
 Sizes default to cases whose inputs exceed the 126 MB L2 while holding well under a
 few GB on the device, so that a multi-pass profiler capture stays short.
@@ -24,7 +27,7 @@ from . import runtime as rt
 def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("case", choices=["gemm_bf16", "gemm_f16", "gemm_s8", "gemm_tf32", "reduce_mean", "reduce_cols", "gather", "gather_elem",
-                                     "matmul_relu_f32", "range"])
+                                     "matmul_relu_f32", "range", "gemm_fp8", "quantize_fp8", "embedding", "embedding_grad"])
     ap.add_argument("--elements", type=int, default=1 << 27)
     ap.add_argument("--m", type=int, default=None)
     ap.add_argument("--n", type=int, default=None)
@@ -38,6 +41,8 @@ def main() -> None:
     ap.add_argument("--beta", type=float, default=1.0, help="GEMM cases: C <- A @ B + beta * C")
     ap.add_argument("--a-col-major", action="store_true", help="gemm_bf16 / gemm_f16: A stored column-major (M contiguous)")
     ap.add_argument("--b-row-major", action="store_true", help="gemm_bf16 / gemm_f16: B stored row-major (N contiguous)")
+    ap.add_argument("--column-scales", action="store_true", help="gemm_fp8: a scale per column of B (the weight gradient) instead of per 128")
+    ap.add_argument("--across", action="store_true", help="quantize_fp8: groups down the columns, transposed result")
     ap.add_argument("--option", action="append", default=[], metavar="NAME=VALUE",
                     help="a launch override for this run, e.g. gemm.group_n=16 (see accb_set_option)")
     a = ap.parse_args()
@@ -46,7 +51,34 @@ def main() -> None:
         rt.set_option(name, int(value))
     dev = torch.device("cuda:0")
     torch.manual_seed(0)
-    if a.case.startswith("gemm_"):
+    if a.case == "gemm_fp8":
+        m, n, k = a.m or 8192, a.n or 8192, a.k or 8192
+        A = torch.randn(m, k, device=dev).to(torch.float8_e4m3fn)
+        B = torch.randn(n, k, device=dev).to(torch.float8_e4m3fn).t()
+        blocks = -(-k // rt.FP8_BLOCK)
+        sa = torch.rand(m, blocks, device=dev) + 0.5
+        sb = (torch.rand(n if a.column_scales else -(-n // rt.FP8_BLOCK), blocks, device=dev) + 0.5).t()
+        C = torch.zeros(m, n, device=dev, dtype=torch.float32 if a.column_scales else torch.bfloat16)
+        for _ in range(a.iters):
+            rt.gemm_fp8(A, B, C, sa, sb, beta=0.0)
+    elif a.case == "quantize_fp8":
+        x = torch.randn(a.rows, a.cols if a.cols != 4096 else 8192, device=dev).to(torch.bfloat16)
+        x = x.t() if a.across else x
+        q = torch.empty(x.shape, device=dev, dtype=torch.float8_e4m3fn)
+        s = torch.empty(x.shape[0], -(-x.shape[1] // rt.FP8_BLOCK), device=dev)
+        for _ in range(a.iters):
+            rt.quantize_fp8(x, q, s)
+    elif a.case.startswith("embedding"):
+        T = (torch.randn(a.table_rows, a.cols, device=dev) * 0.02).to(torch.bfloat16)
+        u = torch.rand(a.indices, device=dev, dtype=torch.float64)          # word frequencies fall like one over the rank
+        ids = (float(a.table_rows) ** u - 1).long().clamp_(0, a.table_rows - 1)
+        rows = torch.empty(a.indices, a.cols, device=dev, dtype=torch.bfloat16)
+        grad = torch.empty(a.table_rows, a.cols, device=dev)
+        for _ in range(a.iters):
+            rt.embedding(T, ids, rows, scale=64.0)
+            if a.case == "embedding_grad":
+                rt.embedding_grad(rows, ids, grad, scale=64.0)
+    elif a.case.startswith("gemm_"):
         m, n, k = a.m or 8192, a.n or 8192, a.k or 8192
         if a.case == "gemm_s8":
             A = torch.randint(-128, 128, (m, k), device=dev, dtype=torch.int8)
