@@ -267,10 +267,20 @@ __device__ void sort_tokens(const void* ids, int* keys0, int* tokens0, int* keys
     if (lane == 0 && bad) { atomicAdd(status + ST_EMBED_COUNT, bad); status[ST_EMBED_ID] = p.launch_id; }
 }
 
-// Words without a token get their final value, zero or beta times the old one, from a kernel of its own that runs beside the
-// sort: it writes most of the table, which HBM bounds, while the sort is bound by latency.  The two are launched with
-// programmatic serialization; the sort starts as soon as every clearing CTA has seen the kernels before it complete, and
-// ends only when the clearing grid has ended, so that what follows the sort follows both.
+__global__ void __launch_bounds__(kSortThreads, 1)
+sort_tokens_kernel(const void* __restrict__ ids, int* keys0, int* tokens0, int* keys1, int* tokens1, int* long_words, int* status, const SortParams p)
+{
+    extern __shared__ int smem[];
+    pdl_enter();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *long_words = 0;
+    sort_tokens(ids, keys0, tokens0, keys1, tokens1, status, p, smem);
+}
+
+// ---------------------------------------------------------------------------------
+// gradient: words without a token
+// ---------------------------------------------------------------------------------
+// They get their final value, zero or beta times the old one, from blocks behind those of the sums in the same grid.
+
 struct ClearParams {
     int64_t stride;
     int dim;
@@ -278,6 +288,35 @@ struct ClearParams {
     float beta;
     int ctas;                    // CTA i owns rows i, i + ctas, ..., so that all CTAs together write one stretch of memory after the other
 };
+
+// One row's value by per_row threads, x of them this one
+template <typename TT>
+__device__ __forceinline__ void clear_row(TT* row, int x, int per_row, const ClearParams& c)
+{
+    constexpr int V = 16 / (int)sizeof(TT);
+    if (c.beta != 0.0f) {
+        for (int i = x; i < c.dim; i += per_row) row[i] = (TT)(c.beta * (float)row[i]);
+    } else if (c.vec) {
+        for (int v = x; v < c.dim / V; v += per_row) reinterpret_cast<uint4*>(row)[v] = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+        // a row that starts or ends within a vector: its whole vectors, and the elements before and after them
+        const int head = min(c.dim, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(TT)), vecs = (c.dim - head) / V;
+        for (int v = x; v < vecs; v += per_row) reinterpret_cast<uint4*>(row + head)[v] = make_uint4(0u, 0u, 0u, 0u);
+        const int tail = head + vecs * V;
+        if (x < head) row[x] = (TT)0.0f;
+        if (tail + x < c.dim && x < V) row[tail + x] = (TT)0.0f;
+    }
+}
+// as many threads side by side as a row has vectors, a power of two from 32 to `most`
+template <typename TT>
+__device__ __forceinline__ int clear_width(const ClearParams& c, int most)
+{
+    constexpr int V = 16 / (int)sizeof(TT);
+    const int width = c.beta == 0.0f ? (c.dim + V - 1) / V : c.dim;
+    int per_row = 32;
+    while (per_row < most && per_row < width) per_row *= 2;
+    return per_row;
+}
 
 // seen: one bit of shared memory for each of the CTA's rows
 template <typename TT, int kThreads>
@@ -295,11 +334,8 @@ __device__ __forceinline__ void clear_rows(TT* table, const void* ids, int part,
         if ((uint32_t)id - at * (uint32_t)c.ctas == (uint32_t)part) atomicOr(seen + at / 32, 1u << (at % 32));
     }
     __syncthreads();
-    // as many threads side by side as a row has vectors: the CTA writes one stretch of memory after the other
-    constexpr int V = 16 / (int)sizeof(TT);
-    const int width = c.beta == 0.0f ? (c.dim + V - 1) / V : c.dim;
-    int per_row = 32;
-    while (per_row < 256 && per_row < width) per_row *= 2;
+    // the CTA writes one stretch of memory after the other
+    const int per_row = clear_width<TT>(c, 256);
     const int sub = threadIdx.x / per_row, x = threadIdx.x % per_row;
     const int groups = kThreads / per_row;                    // a power of two, at most 16: group g takes every groups-th row
     uint32_t every = 0u;
@@ -309,47 +345,49 @@ __device__ __forceinline__ void clear_rows(TT* table, const void* ids, int part,
         while (todo) {
             const int r = w * 32 + __ffs(todo) - 1;
             todo &= todo - 1u;
-            TT* row = table + (part + (int64_t)r * c.ctas) * c.stride;
-            if (c.beta != 0.0f) {
-                for (int i = x; i < c.dim; i += per_row) row[i] = (TT)(c.beta * (float)row[i]);
-            } else if (c.vec) {
-                for (int v = x; v < width; v += per_row) reinterpret_cast<uint4*>(row)[v] = make_uint4(0u, 0u, 0u, 0u);
-            } else {
-                // a row that starts or ends within a vector: its whole vectors, and the elements before and after them
-                const int head = min(c.dim, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(TT)), vecs = (c.dim - head) / V;
-                for (int v = x; v < vecs; v += per_row) reinterpret_cast<uint4*>(row + head)[v] = make_uint4(0u, 0u, 0u, 0u);
-                const int tail = head + vecs * V;
-                if (x < head) row[x] = (TT)0.0f;
-                if (tail + x < c.dim && x < V) row[tail + x] = (TT)0.0f;
-            }
+            clear_row<TT>(table + (part + (int64_t)r * c.ctas) * c.stride, x, per_row, c);
         }
     }
 }
 
-// Two of these an SM: 524 MB of fp32 rows in 80 us; one of 1024 threads an SM took 130.
-constexpr int kClearThreads = 512, kClearWords = 4096;
-
-template <typename TT>
-__global__ void __launch_bounds__(kClearThreads, 2)
-clear_rows_kernel(const void* __restrict__ ids, TT* __restrict__ table, const SortParams p, const ClearParams c)
+// The first place from `lo` of the sorted list whose key is not below `word`, found by a whole warp with 32 probes a step
+__device__ __forceinline__ int first_place(const int* keys, int lo, int n, int word)
 {
-    __shared__ uint32_t seen[kClearWords];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    clear_rows<TT, kClearThreads>(table, ids, (int)blockIdx.x, p, c, seen);
+    int hi = n;
+    while (lo < hi) {
+        const int step = (hi - lo + 31) / 32;
+        const int64_t at = lo + (int64_t)(threadIdx.x % 32) * step;
+        const int below = __popc(__ballot_sync(0xffffffffu, at < hi && keys[at] < word));
+        // probe `below` is not below the word (or behind the range), the one before it is
+        if (below < 32) hi = (int)min((int64_t)hi, lo + (int64_t)below * step);
+        if (below > 0) lo += (below - 1) * step + 1;
+    }
+    return lo;
 }
 
-// beside_clear: a clearing grid comes right before this one in the stream (see above)
-__global__ void __launch_bounds__(kSortThreads, 1)
-sort_tokens_kernel(const void* __restrict__ ids, int* keys0, int* tokens0, int* keys1, int* tokens1, int* long_words, int* status, const SortParams p,
-                   int beside_clear)
+// The clearing of up to 32 rows from the sorted list.  Every warp finds the first place that is not before them and the words
+// in the 32 places from there; where those places do not reach the rows' end, each lane looks for its own word.
+template <typename TT, int kThreads>
+__device__ __forceinline__ void clear_unlisted(TT* table, const int* keys, int n, int first, int rows, int vocab, const ClearParams& c)
 {
-    extern __shared__ int smem[];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (!beside_clear) asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (blockIdx.x == 0 && threadIdx.x == 0) *long_words = 0;
-    sort_tokens(ids, keys0, tokens0, keys1, tokens1, status, p, smem);
-    if (beside_clear) asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int lane = threadIdx.x % 32;
+    rows = min(rows, vocab - first);
+    int lo = first_place(keys, 0, n, first);
+    const int key = lo + lane < n ? keys[lo + lane] : vocab;
+    uint32_t listed = __reduce_or_sync(0xffffffffu, key - first < rows ? 1u << (key - first) : 0u);
+    if (__shfl_sync(0xffffffffu, key, 31) < first + rows) {
+        const int word = first + lane;
+        int hi = n;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (keys[mid] < word) lo = mid + 1; else hi = mid;
+        }
+        listed = __ballot_sync(0xffffffffu, lo < n && keys[lo] == word);
+    }
+    uint32_t todo = ~listed & (rows < 32 ? (1u << rows) - 1u : 0xffffffffu);
+    const int per_row = clear_width<TT>(c, kThreads), sub = threadIdx.x / per_row, x = threadIdx.x % per_row;
+    for (int at = 0; todo; ++at, todo &= todo - 1u)
+        if (at % (kThreads / per_row) == sub) clear_row<TT>(table + (int64_t)(first + __ffs(todo) - 1) * c.stride, x, per_row, c);
 }
 
 // ---------------------------------------------------------------------------------
@@ -363,7 +401,14 @@ sort_tokens_kernel(const void* __restrict__ ids, int* keys0, int* tokens0, int* 
 
 constexpr int kChunk = 32;
 constexpr int kSumThreads = 128;
-constexpr int kSumUnroll = 2;
+// A thread has two rows on their way with sixteen blocks an SM, eight with four blocks.  Up to kSumDeep blocks of sums an SM, the
+// time of one block counts: 6271 tokens of 112 columns took 47 us with two rows, 38 with eight; beyond, the blocks do each
+// other's waiting (16384 tokens of 4096 columns: 132 us with two rows, 141 with eight).
+constexpr int kSumDeep = 6;
+// The blocks behind those of the sums give words without a token their value, as many rows each as make kClearBytes, so
+// that all of them together write one stretch of memory after the other and the sums' loads have stores beside them: 16384
+// tokens into 32000 x 4096 fp32 take 137 us at 32 KB a block, 197 at 512 KB, 160 with the clearing beside the sort instead.
+constexpr int64_t kClearBytes = 32768;
 
 struct SumParams {
     int n, vocab, dim;
@@ -371,6 +416,7 @@ struct SumParams {
     float scale, beta;
     int chunks;
     int slabs;
+    int clear_rows;              // of words without a token that a block behind those of the sums looks after: up to 32
 };
 
 template <typename TT, int E>
@@ -389,12 +435,16 @@ __device__ __forceinline__ void write_sum(TT* table, int64_t word, int64_t strid
     *dst = y;
 }
 
-template <typename TT, typename TR, int E>
-__global__ void __launch_bounds__(kSumThreads, 16)
+template <typename TT, typename TR, int E, int U>
+__global__ void __launch_bounds__(kSumThreads, U == 2 ? 16 : 4)
 sum_rows_kernel(const TR* __restrict__ rows, const int* __restrict__ keys, const int* __restrict__ tokens, TT* __restrict__ table,
-                float* __restrict__ partial, int* __restrict__ long_words, const SumParams p)
+                float* __restrict__ partial, int* __restrict__ long_words, const SumParams p, const ClearParams c)
 {
     pdl_enter();
+    if ((int)blockIdx.x >= p.chunks * p.slabs) {
+        clear_unlisted<TT, kSumThreads>(table, keys, p.n, ((int)blockIdx.x - p.chunks * p.slabs) * p.clear_rows, p.clear_rows, p.vocab, c);
+        return;
+    }
     const int chunk = blockIdx.x / p.slabs, slab = blockIdx.x % p.slabs;
     const int i0 = chunk * kChunk, i1 = min(p.n, i0 + kChunk);
     __shared__ int key[3 * kChunk + 1];                      // places i0 - kChunk ..
@@ -447,20 +497,20 @@ sum_rows_kernel(const TR* __restrict__ rows, const int* __restrict__ keys, const
     const uint64_t ends = (uint64_t)__ballot_sync(0xffffffffu, k[lane] != k[lane + 1]) | (uint64_t)__ballot_sync(0xffffffffu, k[lane + kChunk] != k[lane + kChunk + 1]) << 32;
     const int col = (slab * kSumThreads + threadIdx.x) * E;
     if (col >= p.dim || first >= last) return;
-    // kSumUnroll rows are always on their way: a place's register takes the row kSumUnroll places on as soon as it is added
+    // U rows are always on their way: a place's register takes the row U places on as soon as it is added
     const TR* src = rows + col;
-    Vec<TR, E> x[kSumUnroll];
+    Vec<TR, E> x[U];
 #pragma unroll
-    for (int u = 0; u < kSumUnroll; ++u) x[u] = *reinterpret_cast<const Vec<TR, E>*>(src + row_at[min(first + u, last - 1)]);
+    for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const Vec<TR, E>*>(src + row_at[min(first + u, last - 1)]);
     float acc[E] = {};
-    for (int j0 = first; j0 < last; j0 += kSumUnroll) {
+    for (int j0 = first; j0 < last; j0 += U) {
 #pragma unroll
-        for (int u = 0; u < kSumUnroll; ++u) {
+        for (int u = 0; u < U; ++u) {
             const int j = j0 + u;
             if (j >= last) break;
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[e] += (float)x[u].v[e];
-            if (j + kSumUnroll < last) x[u] = *reinterpret_cast<const Vec<TR, E>*>(src + row_at[j + kSumUnroll]);
+            if (j + U < last) x[u] = *reinterpret_cast<const Vec<TR, E>*>(src + row_at[j + U]);
             if (j + 1 == last || (ends >> j & 1u)) {
                 const bool head = first_long && k[j] == k_first, tail = last_long && j + 1 == last;
                 if (head || tail) {
@@ -498,17 +548,7 @@ join_rows_kernel(const float* __restrict__ partial, const int* __restrict__ keys
     for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
         const int chunk = long_words[1 + w / col_blocks], col = ((int)(w % col_blocks) * kJoinCols + x) * E;
         const int word = keys[chunk * kChunk + kChunk - 1];
-        // the first place behind the word, found by each warp for itself with 32 probes a step of the sorted list
-        int lo = chunk * kChunk + kChunk, hi = p.n;
-        while (lo < hi) {
-            const int step = (hi - lo + 31) / 32;
-            const int64_t at = lo + (int64_t)x * step;
-            const int inside = __popc(__ballot_sync(0xffffffffu, at < hi && keys[at] <= word));
-            // probe `inside` lies behind the word (or the range), the one before it does not
-            if (inside < 32) hi = (int)min((int64_t)hi, lo + (int64_t)inside * step);
-            if (inside > 0) lo += (inside - 1) * step + 1;
-        }
-        const int last_chunk = (lo - 1) / kChunk;
+        const int last_chunk = (first_place(keys, chunk * kChunk + kChunk, p.n, word + 1) - 1) / kChunk;
         Vec<float, E> acc = {};
         if (col < p.dim) {
 #pragma unroll 8
@@ -539,17 +579,18 @@ join_rows_kernel(const float* __restrict__ partial, const int* __restrict__ keys
 // it is its word's first token; else it collects the word's tokens in order and adds their rows: a thread one vector of
 // columns, or, for more than kFewSplit tokens, kFewLanes threads a vector, each a kFewLanes-th of the list, whose
 // sums are added in lane order.  Blocks behind those give words without a token their value.
-constexpr int kFewTokens = 1024, kFewThreads = 256, kFewLanes = 8, kFewSplit = 16, kFewUnroll = 8;
+// Above kFewTokens the list is sorted: 1598 tokens of 144 columns take 18 us here and 46 sorted, 3708 of 128 columns 45 and 31.
+constexpr int kFewTokens = 2048, kFewThreads = 256, kFewLanes = 8, kFewSplit = 16, kFewUnroll = 8;
 
-template <typename TT, typename TR, int E>
+template <typename TT, typename TR, int E, int kRounds>
 __global__ void __launch_bounds__(kFewThreads)
 few_tokens_kernel(const TR* __restrict__ rows, const void* __restrict__ ids, TT* __restrict__ table, int* __restrict__ status, const SortParams sp,
                   const ClearParams c, const SumParams p)
 {
     pdl_enter();
-    constexpr int kWarps = kFewThreads / 32, kRounds = kFewTokens / kFewThreads;
-    __shared__ uint32_t list[kFewTokens];
-    __shared__ int count[kRounds][kWarps];
+    constexpr int kWarps = kFewThreads / 32;
+    __shared__ uint32_t list[kRounds * kFewThreads];
+    __shared__ int count[(kRounds * kWarps + 31) / 32 * 32];        // of a round and warp, in list order
     __shared__ float part[kFewLanes][kFewThreads / kFewLanes][E + 1];
     const int sum_blocks = sp.n * p.slabs;
     if ((int)blockIdx.x >= sum_blocks) {
@@ -572,17 +613,24 @@ few_tokens_kernel(const TR* __restrict__ rows, const void* __restrict__ ids, TT*
         const bool same = i < sp.n && load_id(ids, i, sp.id_bytes) == word;
         earlier |= same && i < token;
         mine[r] = __ballot_sync(0xffffffffu, same);
-        if (lane == 0) count[r][warp] = __popc(mine[r]);
+        if (lane == 0) count[r * kWarps + warp] = __popc(mine[r]);
     }
     if (__syncthreads_or(earlier)) return;
+    // every warp adds the counts up for itself
     int n = 0;
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r)
+    for (int r0 = 0; r0 < kRounds; r0 += 32 / kWarps) {
+        const int own = r0 * kWarps + lane < kRounds * kWarps ? count[r0 * kWarps + lane] : 0;
+        int sum = own;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w == warp && (mine[r] >> lane & 1u)) list[n + __popc(mine[r] & ((1u << lane) - 1u))] = (uint32_t)(r * kFewThreads + threadIdx.x);
-            n += count[r][w];
+        for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += v; }
+#pragma unroll
+        for (int r = r0; r < kRounds && r < r0 + 32 / kWarps; ++r) {
+            const int before = n + __shfl_sync(0xffffffffu, sum - own, (r - r0) * kWarps + warp);
+            if (mine[r] >> lane & 1u) list[before + __popc(mine[r] & ((1u << lane) - 1u))] = (uint32_t)(r * kFewThreads + threadIdx.x);
         }
+        n += __shfl_sync(0xffffffffu, sum, 31);
+    }
     __syncthreads();
     if (n <= kFewSplit) {
         const int col = (slab * kFewThreads + threadIdx.x) * E;
@@ -662,7 +710,7 @@ ClearParams clear_params(const accb_embedding_desc& d, const void* table, int64_
     return c;
 }
 
-cudaError_t launch_sort(const EmbeddingLaunch& l, const SortParams& s, int* keys0, int* tokens0, int* keys1, int* tokens1, int* long_words, bool beside_clear)
+cudaError_t launch_sort(const EmbeddingLaunch& l, const SortParams& s, int* keys0, int* tokens0, int* keys1, int* tokens1, int* long_words)
 {
     static std::atomic<bool> opted[64];
     if (l.device >= 64 || !opted[l.device].load(std::memory_order_acquire)) {
@@ -670,17 +718,16 @@ cudaError_t launch_sort(const EmbeddingLaunch& l, const SortParams& s, int* keys
         if (e != cudaSuccess) return e;
         if (l.device < 64) opted[l.device].store(true, std::memory_order_release);
     }
-    const unsigned cluster = s.n <= 2048 ? 1 : s.n <= 4096 ? 2 : s.n <= 8192 ? 4 : kSortCluster;
     const bool pdl = options().stream_pdl != 0;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(cluster); cfg.blockDim = dim3(kSortThreads); cfg.dynamicSmemBytes = kSortSmem; cfg.stream = l.stream;
+    cfg.gridDim = dim3(kSortCluster); cfg.blockDim = dim3(kSortThreads); cfg.dynamicSmemBytes = kSortSmem; cfg.stream = l.stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.x = kSortCluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, sort_tokens_kernel, l.ids, keys0, tokens0, keys1, tokens1, long_words, l.status, s, beside_clear ? 1 : 0);
+    return cudaLaunchKernelEx(&cfg, sort_tokens_kernel, l.ids, keys0, tokens0, keys1, tokens1, long_words, l.status, s);
 }
 
 template <typename TT, typename TR>
@@ -709,14 +756,17 @@ int launch_grad(const EmbeddingLaunch& l, const void* rows, void* table, const c
 
     if (n <= kFewTokens) {
         // a few rows a clearing block, four blocks an SM, and no more rows than a block's bit list holds
-        const int64_t most = (int64_t)kFewTokens * 32;
+        const int rounds = n <= 2 * kFewThreads ? 2 : n <= 4 * kFewThreads ? 4 : 8;
+        const int64_t most = (int64_t)rounds * kFewThreads * 32;
         int64_t ctas = clear ? (d.vocab + 7) / 8 : 0;
         if (ctas > 4 * l.num_sms) ctas = 4 * l.num_sms;
         if (clear && (d.vocab + most - 1) / most > ctas) ctas = (d.vocab + most - 1) / most;
         const ClearParams c = clear_params<TT>(d, table, ctas > 0 ? ctas : 1);
         const dim3 grid((unsigned)(n * p.slabs + ctas)), block(kFewThreads);
-        const cudaError_t e = vec ? launch_pdl(few_tokens_kernel<TT, TR, E>, grid, block, l.stream, (const TR*)rows, l.ids, (TT*)table, l.status, s, c, p)
-                                  : launch_pdl(few_tokens_kernel<TT, TR, 1>, grid, block, l.stream, (const TR*)rows, l.ids, (TT*)table, l.status, s, c, p);
+        auto kernel = rounds == 2 ? (vec ? few_tokens_kernel<TT, TR, E, 2> : few_tokens_kernel<TT, TR, 1, 2>)
+                    : rounds == 4 ? (vec ? few_tokens_kernel<TT, TR, E, 4> : few_tokens_kernel<TT, TR, 1, 4>)
+                                  : (vec ? few_tokens_kernel<TT, TR, E, 8> : few_tokens_kernel<TT, TR, 1, 8>);
+        const cudaError_t e = launch_pdl(kernel, grid, block, l.stream, (const TR*)rows, l.ids, (TT*)table, l.status, s, c, p);
         if (e != cudaSuccess) return cuda_failed(e);
         note_launches(1);
         return 1;
@@ -732,23 +782,23 @@ int launch_grad(const EmbeddingLaunch& l, const void* rows, void* table, const c
     const int* keys = (s.passes & 1) ? keys0 : keys1;
     const int* tokens = (s.passes & 1) ? tokens0 : tokens1;
     cudaError_t e = cudaSuccess;
-    if (clear) {
-        const int64_t most = (int64_t)kClearWords * 32, need = (d.vocab + most - 1) / most;
-        const int64_t ctas = need > 2 * l.num_sms ? need : 2 * l.num_sms;
-        e = launch_pdl(clear_rows_kernel<TT>, dim3((unsigned)ctas), dim3(kClearThreads), l.stream, l.ids, (TT*)table, s, clear_params<TT>(d, table, ctas));
-    }
-    if (e == cudaSuccess) e = launch_sort(l, s, keys0, tokens0, keys1, tokens1, long_words, clear);
-    const dim3 grid((unsigned)blocks), block(kSumThreads);
-    if (e == cudaSuccess)
-        e = vec ? launch_pdl(sum_rows_kernel<TT, TR, E>, grid, block, l.stream, (const TR*)rows, keys, tokens, (TT*)table, partial, long_words, p)
-                : launch_pdl(sum_rows_kernel<TT, TR, 1>, grid, block, l.stream, (const TR*)rows, keys, tokens, (TT*)table, partial, long_words, p);
+    const ClearParams c = clear_params<TT>(d, table, 1);
+    p.clear_rows = 32;
+    while (p.clear_rows > 1 && p.clear_rows * d.dim * (int64_t)sizeof(TT) > kClearBytes) p.clear_rows /= 2;
+    if (e == cudaSuccess) e = launch_sort(l, s, keys0, tokens0, keys1, tokens1, long_words);
+    const int64_t rest = clear ? (d.vocab + p.clear_rows - 1) / p.clear_rows : 0;
+    if (blocks + rest > 0x7fffffff) { temp_free(ws, l.stream); return cuda_failed(cudaErrorInvalidConfiguration); }
+    const dim3 grid((unsigned)(blocks + rest)), block(kSumThreads);
+    const bool deep = blocks <= kSumDeep * (int64_t)l.num_sms;
+    auto sum = vec ? (deep ? sum_rows_kernel<TT, TR, E, 8> : sum_rows_kernel<TT, TR, E, 2>) : (deep ? sum_rows_kernel<TT, TR, 1, 8> : sum_rows_kernel<TT, TR, 1, 2>);
+    if (e == cudaSuccess) e = launch_pdl(sum, grid, block, l.stream, (const TR*)rows, keys, tokens, (TT*)table, partial, long_words, p, c);
     if (e == cudaSuccess)
         e = launch_pdl(vec ? join_rows_kernel<TT, 4> : join_rows_kernel<TT, 1>, dim3((unsigned)(8 * l.num_sms)), dim3(kJoinCols * kJoinLanes), l.stream,
                        (const float*)partial, keys, (const int*)long_words, (TT*)table, p);
     temp_free(ws, l.stream);
     if (e != cudaSuccess) return cuda_failed(e);
-    note_launches(clear ? 4 : 3);
-    return clear ? 4 : 3;
+    note_launches(3);
+    return 3;
 }
 
 template <template <typename, typename> class F, typename... Args>

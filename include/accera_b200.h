@@ -242,7 +242,7 @@ int accb_gather_rank2_dims(int64_t d0, int64_t d1, int64_t i0, int64_t i1, int32
  * An id outside [0, vocab) is not dereferenced: its row is zero-filled (lookup) or left out (gradient) and
  * ACCB_ERR_INDEX is reported, from this call for host pointers and from the next accb_synchronize() for device
  * pointers.  Neither array may overlap the other.  A device-pointer accb_embedding_grad of more than
- * 1024 tokens takes its workspace (16 bytes a token and some partial sums) from a stream-ordered pool of the library, so calls on
+ * 2048 tokens takes its workspace (16 bytes a token and some partial sums) from a stream-ordered pool of the library, so calls on
  * several streams, and captured graphs, do not share it.
  * tokens is at most 2^30, vocab below 2^31 - 1, dim at most 2^20.
  */

@@ -131,7 +131,7 @@ def test_gradient_equals_the_formula(kind, tokens, vocab, dim):
 
 @pytest.mark.parametrize("tg,tt", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "bf16"), ("f16", "f32")])
 @pytest.mark.parametrize("beta,padding", [(0.0, None), (1.0, 2), (-0.5, 0), (1.0, None)])
-@pytest.mark.parametrize("tokens", [700, 1500])                           # both gradient kernels: few tokens, sorted tokens
+@pytest.mark.parametrize("tokens", [300, 700, 1500, 2500])                # few tokens by 512, 1024 and 2048, and sorted tokens
 def test_gradient_types_beta_padding_and_strides(tokens, tg, tt, beta, padding):
     ids = _ids("zipf", tokens, 90, 5)
     ids[::50] = 2
@@ -148,6 +148,23 @@ def test_gradient_types_beta_padding_and_strides(tokens, tg, tt, beta, padding):
         rt.synchronize()
         _check_grad(table[:, lead:lead + 80].cpu(), want, err, (tg, tt, beta, padding, pad_cols))
         assert (table[:, :lead] == 4).all() and (table[:, lead + 80:] == 4).all()
+
+
+@pytest.mark.parametrize("tokens", [1, 511, 512, 513, 1024, 1025, 2047, 2048, 2049, 6000])
+@pytest.mark.parametrize("vocab,dim", [(33, 40), (1000, 20), (4097, 1), (300, 5000), (70, 20000)])
+@pytest.mark.parametrize("beta", [0.0, 0.5])
+def test_words_without_a_token_between_frequent_ones(tokens, vocab, dim, beta):
+    if tokens * dim > 2 ** 24:
+        tokens = 2049 if tokens > 2048 else 600                           # (small tables of long rows: enough with these)
+    ids = torch.arange(tokens) % 3 * 11 + torch.arange(tokens) % 7 // 6   # words 0, 1, 11, 12, 22, 23, often; the rest never but for the last
+    ids[-1] = vocab - 1
+    g = torch.randint(-3, 4, (tokens, dim)).to(torch.bfloat16)
+    old = torch.randint(-8, 9, (vocab, dim)).float()
+    want = torch.zeros(vocab, dim, dtype=torch.float64).index_add_(0, ids, g.double()) + beta * old.double()
+    got = old.cuda()
+    rt.embedding_grad(g.cuda(), ids.cuda(), got, beta=beta)
+    rt.synchronize()
+    assert torch.equal(got.cpu().double(), want)                          # sums of small whole numbers: exact
 
 
 def test_words_without_a_token_keep_their_bytes_with_beta_one():
