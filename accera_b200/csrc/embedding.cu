@@ -41,7 +41,7 @@ struct LookupParams {
     uint32_t vocab;
     uint32_t vecs;              // vectors in a row
     int shift;                  // log2 of the threads that share a row
-    uint32_t pairs;             // blocks that share a row: each thread takes two vectors of it; 0: one vector of two rows
+    uint32_t parts;             // blocks that share a row: each thread takes U vectors of it; 0: one vector of U rows
     float scale;
     int id_bytes;
     int launch_id;
@@ -54,49 +54,55 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int64_t t, int id_by
     return id_bytes == 8 ? __ldg((const long long*)ids + t) : (int64_t)__ldg((const int*)ids + t);
 }
 
-// A thread moves two vectors, with both loads in flight: two of its row, or, where a row has no more vectors than threads, one
-// each of two rows.  Threads find their row without a division, and the loads in flight come from eight resident blocks an
-// SM: 16384 rows of 4096 bf16 take 44 us with a division a vector, 58 with four vectors a thread (and three blocks an SM).
-template <typename TT, typename TR, int E>
-__global__ void __launch_bounds__(kLookupBlock, 8)
+// A thread moves U vectors, with all loads in flight: U of its row, or, where a row has no more vectors than threads, one
+// each of U rows.  Threads find their row without a division.  U = 2 for vectors of 16 bytes, the loads in flight coming from
+// eight resident blocks an SM: 16384 rows of 4096 bf16 take 40 us, 44 with a division a vector, 58 with four vectors a thread (and
+// three blocks an SM).  U = 8 for rows that have to go by single elements: 9968 rows of 3283 fp16 take 93 us, with U = 2 142.
+template <typename TT, typename TR, int E, int U>
+__global__ void __launch_bounds__(kLookupBlock, U == 2 ? 8 : 4)
 embedding_kernel(const TT* __restrict__ table, const void* __restrict__ ids, TR* __restrict__ rows, int* __restrict__ status,
                  const LookupParams p)
 {
     pdl_enter();
     const uint32_t x = threadIdx.x & ((1u << p.shift) - 1u);
     const int groups = kLookupBlock >> p.shift, sub = threadIdx.x >> p.shift;
-    int64_t row[2];
-    uint32_t vec[2];
-    if (p.pairs) {
-        const uint32_t part = blockIdx.x % p.pairs;
-        row[0] = row[1] = (int64_t)(blockIdx.x / p.pairs) * groups + sub;
-        vec[0] = x + ((2 * part) << p.shift);
-        vec[1] = vec[0] + (1u << p.shift);
+    int64_t row0;
+    uint32_t vec0, vec_step;
+    int row_step;
+    if (p.parts) {
+        row0 = (int64_t)(blockIdx.x / p.parts) * groups + sub;
+        row_step = 0;
+        vec0 = x + ((U * (blockIdx.x % p.parts)) << p.shift);
+        vec_step = 1u << p.shift;
     } else {
-        row[0] = (int64_t)blockIdx.x * (2 * groups) + sub;
-        row[1] = row[0] + groups;
-        vec[0] = vec[1] = x;
+        row0 = (int64_t)blockIdx.x * (U * groups) + sub;
+        row_step = groups;
+        vec0 = x;
+        vec_step = 0;
     }
-    Vec<TT, E> v[2];
-    bool in[2], ok[2];
+    Vec<TT, E> v[U];
+    bool ok[U];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        in[u] = row[u] < p.tokens && vec[u] < p.vecs;
+    for (int u = 0; u < U; ++u) {
+        const int64_t row = row0 + u * row_step;
+        const uint32_t vec = vec0 + u * vec_step;
         ok[u] = false;
-        if (in[u]) {
-            const int64_t id = load_id(ids, row[u], p.id_bytes);
+        if (row < p.tokens && vec < p.vecs) {
+            const int64_t id = load_id(ids, row, p.id_bytes);
             ok[u] = (uint64_t)id < p.vocab;
-            if (!ok[u] && vec[u] == 0) { atomicAdd(status + ST_EMBED_COUNT, 1); status[ST_EMBED_ID] = p.launch_id; }
-            if (ok[u]) v[u] = *reinterpret_cast<const Vec<TT, E>*>(table + id * p.table_stride + vec[u] * (int64_t)E);
+            if (!ok[u] && vec == 0) { atomicAdd(status + ST_EMBED_COUNT, 1); status[ST_EMBED_ID] = p.launch_id; }
+            if (ok[u]) v[u] = *reinterpret_cast<const Vec<TT, E>*>(table + id * p.table_stride + vec * (int64_t)E);
         }
     }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        if (!in[u]) continue;
+    for (int u = 0; u < U; ++u) {
+        const int64_t row = row0 + u * row_step;
+        const uint32_t vec = vec0 + u * vec_step;
+        if (row >= p.tokens || vec >= p.vecs) continue;
         Vec<TR, E> y;
 #pragma unroll
         for (int e = 0; e < E; ++e) y.v[e] = ok[u] ? (TR)((float)v[u].v[e] * p.scale) : (TR)0.0f;
-        store_streaming<TR, E>(rows + row[u] * p.rows_stride + vec[u] * (int64_t)E, y);
+        store_streaming<TR, E>(rows + row * p.rows_stride + vec * (int64_t)E, y);
     }
 }
 
@@ -114,21 +120,23 @@ cudaError_t launch_lookup(const EmbeddingLaunch& l, const void* table, void* row
     p.vocab = (uint32_t)d.vocab;
     p.vecs = (uint32_t)(vec ? d.dim / E : d.dim);
     p.scale = d.scale; p.id_bytes = d.id_bytes; p.launch_id = l.launch_id;
-    // threads to a row: the power of two that leaves the fewest of them idle, the larger one of equals
+    const uint32_t each = vec ? 2 : 8;
+    // threads to a row: the power of two that leaves the fewest of them idle, the larger one of equals; all of a block for
+    // long rows of single elements, whose parts by fewer threads share too many lines (3283 fp16: 283 us by 64 threads)
     p.shift = 0;
     uint32_t best = 0;
-    for (int shift = 0; shift <= 8; ++shift) {
-        const uint32_t t = 1u << shift, turns = (p.vecs + t - 1) / t, used = (uint32_t)((uint64_t)p.vecs * 1024 / ((uint64_t)(turns == 1 ? 1 : (turns + 1) / 2 * 2) * t));
+    for (int shift = !vec && p.vecs > 1024 ? 8 : 0; shift <= 8; ++shift) {
+        const uint32_t t = 1u << shift, turns = (p.vecs + t - 1) / t, used = (uint32_t)((uint64_t)p.vecs * 1024 / ((uint64_t)(turns == 1 ? 1 : (turns + each - 1) / each * each) * t));
         if (used >= best) { best = used; p.shift = shift; }
     }
     const uint32_t turns = (p.vecs + (1u << p.shift) - 1) >> p.shift;
-    p.pairs = turns == 1 ? 0 : (turns + 1) / 2;
+    p.parts = turns == 1 ? 0 : (turns + each - 1) / each;
     const int64_t groups = kLookupBlock >> p.shift;
-    const int64_t blocks = p.pairs ? (d.tokens + groups - 1) / groups * p.pairs : (d.tokens + 2 * groups - 1) / (2 * groups);
+    const int64_t blocks = p.parts ? (d.tokens + groups - 1) / groups * p.parts : (d.tokens + each * groups - 1) / (each * groups);
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
     const dim3 grid((unsigned)blocks), block(kLookupBlock);
-    return vec ? launch_pdl(embedding_kernel<TT, TR, E>, grid, block, l.stream, (const TT*)table, l.ids, (TR*)rows, l.status, p)
-               : launch_pdl(embedding_kernel<TT, TR, 1>, grid, block, l.stream, (const TT*)table, l.ids, (TR*)rows, l.status, p);
+    return vec ? launch_pdl(embedding_kernel<TT, TR, E, 2>, grid, block, l.stream, (const TT*)table, l.ids, (TR*)rows, l.status, p)
+               : launch_pdl(embedding_kernel<TT, TR, 1, 8>, grid, block, l.stream, (const TT*)table, l.ids, (TR*)rows, l.status, p);
 }
 
 // ---------------------------------------------------------------------------------
