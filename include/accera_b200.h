@@ -273,7 +273,7 @@ int accb_embedding_grad(const accb_embedding_desc* desc, const void* rows, const
  * x is rows x cols (ACCB_F32, ACCB_F16, ACCB_BF16) with any positive strides; a transposed view (strides {1, ld}) gives
  * the transposed result with its groups along the other direction, at the same speed.  q is row-major with q_stride elements
  * between rows; scales is ceil(rows / block_rows) x ceil(cols / 128) with any positive strides.  The last group of a
- * row or column may be partial.  Host or device pointers as for accb_gemm; no workspace.
+ * row or column may be partial.  q and scales must not overlap x.  Host or device pointers as for accb_gemm; no workspace.
  */
 typedef struct accb_quantize_fp8_desc {
     int64_t rows, cols;
@@ -300,8 +300,9 @@ int accb_quantize_fp8(const accb_quantize_fp8_desc* desc, const void* x, void* q
  *
  * a_scales is ceil(M / a_block) x ceil(K / 128), b_scales ceil(K / 128) x ceil(N / b_block), a_block and b_block each
  * 1 (a scale per row of A / column of B) or 128, any positive strides; any fp32 value may be a scale.  Infinities
- * and NaN of a block stay with their row or column, also through the ReLU.  Activations (a_block = 1) times weights (b_block = 128) is the forward product and, with the
- * weights' other direction contiguous, the gradient of its input; 1 and 1 is the gradient of its weights.
+ * and NaN of a block stay with their row or column, also through the ReLU.  Activations (a_block = 1) times weights
+ * (b_block = 128) is the forward product and, with the weights' other direction contiguous, the gradient of its input; 1 and 1 is
+ * the gradient of its weights.  C must not overlap anything that is read.
  *
  * Layouts: on the tensor cores each operand is contiguous along K or along its other direction; C has any strides.
  * Operands whose rows are not 16-byte aligned are copied into aligned rows first, and few-tile problems keep fp32 sums of
