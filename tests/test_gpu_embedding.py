@@ -54,7 +54,7 @@ def _check_grad(got, want, err32, what):
     assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, first at {bad.nonzero()[0].tolist()}: got {got[bad][0]} want {want[bad][0]}"
 
 
-@pytest.mark.parametrize("tokens,dim", [(1, 4096), (8, 8), (33, 1), (257, 100), (1000, 129), (3, 20000)])
+@pytest.mark.parametrize("tokens,dim", [(1, 4096), (8, 8), (33, 1), (257, 100), (1000, 129), (3, 20000), (19, 1023), (10, 1025), (7, 3283), (2, 20001)])
 @pytest.mark.parametrize("tt,tr", [("bf16", "bf16"), ("f32", "bf16"), ("f16", "f32"), ("f32", "f32")])
 def test_lookup_equals_the_formula(tokens, dim, tt, tr):
     g = torch.Generator().manual_seed(tokens + dim)
