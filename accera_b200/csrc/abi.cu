@@ -169,11 +169,11 @@ int decode_status(const int* w, int what, int id, bool* clear_gemm, bool* clear_
     if (gemm_failed && gemm_mine) {
         static const char* sites[] = { "?", "producer waiting for a free stage", "MMA waiting for operands",
                                        "MMA waiting for a free accumulator", "epilogue waiting for the accumulator",
-                                       "forwarding CTA waiting for a tile" };
+                                       "forwarding CTA waiting for a tile", "epilogue waiting for scales" };
         const int site = (w[ST_GEMM_SITE] >> 24) & 0xff;
         char buf[256];
         snprintf(buf, sizeof buf, "tcgen05 GEMM (launch %d): bounded wait ran out (%s, block %d, step %d; %d wait(s) in all); "
-                 "results are invalid", w[ST_GEMM_ID], site >= 1 && site <= 5 ? sites[site] : sites[0],
+                 "results are invalid", w[ST_GEMM_ID], site >= 1 && site <= 6 ? sites[site] : sites[0],
                  w[ST_GEMM_SITE] & 0xffffff, w[ST_GEMM_STEP], w[ST_GEMM_COUNT]);
         *msg = buf;
         *clear_gemm = true;
@@ -679,6 +679,7 @@ int accb_set_option(const char* name, int64_t value)
     else if (n == "gemm.split_k") o.gemm_split_k = v < 0 ? -1 : (int)v;
     else if (n == "gemm_fp8.kernel") { if (value < 0 || value > 2) return fail(ACCB_ERR_ARG, "accb_set_option: gemm_fp8.kernel is 0, 1 or 2"); o.gemm_fp8_kernel = v; }
     else if (n == "gemm_fp8.slices") { if (value != 0 && value != 1 && value != 2 && value != 4 && value != 8) return fail(ACCB_ERR_ARG, "accb_set_option: gemm_fp8.slices is 0, 1, 2, 4 or 8"); o.gemm_fp8_slices = v; }
+    else if (n == "gemm_fp8.test_drop_scales") o.gemm_fp8_test_drop_scales = v ? 1 : 0;
     else if (n == "stream_kernels.pdl") o.stream_pdl = v < 0 ? -1 : (v ? 1 : 0);
     else if (n == "gemm.c_in") o.gemm_c_in = v < 0 ? -1 : (v ? 1 : 0);
     else if (n == "gemm.verbose") o.gemm_verbose = v ? 1 : 0;

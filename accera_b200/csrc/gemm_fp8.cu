@@ -64,6 +64,7 @@ struct F8Params {
     int launch_id;
     unsigned long long wait_ns;
     int drop_commit;                        // self-test of the time-out path: the commit of the last block's MMAs is left out
+    int drop_scales;                        // the same: the arrival of a tile's last scales is left out
 };
 
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi)
@@ -548,7 +549,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 const bool whole = blocks == Plan::kGroup && kb0 % Plan::kGroup == 0;
                 copy(p.sa, row_a, p.m, 32, p.a_shift, p.sa_row, p.sa_kb, 4, 0, p.sa_vec && whole);
                 if (COLS || lane < 2) copy(p.sb, col_b, p.n, 32, p.b_shift, p.sb_col, p.sb_kb, COLS ? 8 : 1, kRowsX, p.sb_vec && whole);
-                copies_arrive(scale_full_bar(r));
+                if (!(p.drop_scales && kb0 + Plan::kGroup >= kb_end)) copies_arrive(scale_full_bar(r));
                 if (++r == Plan::kSlots) { r = 0; rph ^= 1u; }
             }
         }
@@ -607,11 +608,18 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             for (int kb = 0; kb < num_kb; ++kb, ++g) {
                 const int buf = g & 1, in_group = kb % Plan::kGroup;
                 const uint32_t taddr = taddr0 + (uint32_t)(buf * Plan::kBN);
-                if (in_group == 0) ok = mbar_wait(scale_full_bar(r), rph, wctx, SITE_EPI_TMEM_FULL, kb);
-                if (!loading) {
-                    ok = ok && mbar_wait(done_bar(s), ph, wctx, SITE_EPI_TMEM_FULL, kb);
+                // The lanes leave a wait one by one; the vote after it brings them together for the warp-wide tcgen05.ld and wait::ld,
+                // and all of them stay or leave.  With the block's load already on its way, only a new slot of scales is waited for.
+                if (in_group == 0 || !loading) {
+                    ok = in_group != 0 || mbar_wait(scale_full_bar(r), rph, wctx, SITE_EPI_SCALES, kb);
+                    ok = ok && (loading || mbar_wait(done_bar(s), ph, wctx, SITE_EPI_TMEM_FULL, kb));
                     ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
+                    if (!ok) {
+                        if (loading) tmem_wait_ld(x0);           // no load may be in flight when TMEM is given back
+                        break;
+                    }
+                }
+                if (!loading) {
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     if constexpr (COLS) tmem_ld_pairs(taddr, x0);
                     else tmem_ld32(taddr, x0);
@@ -847,7 +855,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 #pragma unroll
             for (int i = 0; i < kColLoads; ++i)
                 if (i * 32 + lane < BN) copy_scale(sc + (kRowsX + i * 32 + lane) * 4, src_t[i] + kb * p.sa_kb, in_t[i]);
-            copies_arrive(scale_full_bar(r));
+            if (!(p.drop_scales && kb == kb_end - 1)) copies_arrive(scale_full_bar(r));
             if (++r == kRing) { r = 0; rph ^= 1u; }
         }
         if (!ok && lane == 0) gave_up[0] = 1u;
@@ -883,7 +891,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         uint32_t bph = 0, rph = 0;
         bool ok = true;
         for (int kb = kb_begin; kb < kb_end; ++kb) {
-            ok = mbar_wait(scale_full_bar(r), rph, wctx, SITE_EPI_TMEM_FULL, kb) && mbar_wait(tmem_full_bar(b), bph, wctx, SITE_EPI_TMEM_FULL, kb);
+            ok = mbar_wait(scale_full_bar(r), rph, wctx, SITE_EPI_SCALES, kb) && mbar_wait(tmem_full_bar(b), bph, wctx, SITE_EPI_TMEM_FULL, kb);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -1127,6 +1135,7 @@ int launch_gemm_fp8(const GemmFp8Launch& g0, const char** err)
     p.status = g.status; p.launch_id = g.launch_id;
     const Options& o = options();
     p.drop_commit = o.gemm_test_drop_commit;
+    p.drop_scales = o.gemm_fp8_test_drop_scales;
     p.wait_ns = o.gemm_wait_limit_us > 0 ? (unsigned long long)o.gemm_wait_limit_us * 1000ull : 1000000000ull;
 
     // Which kernel, and how many slices of K, by estimated microseconds, fitted to measured launches (graph replays).

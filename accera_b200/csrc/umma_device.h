@@ -16,7 +16,7 @@ constexpr uint32_t kPeerMask = 0xFEFFFFFFu;  // clears the CTA-rank bit of a sha
 enum { KIND_F16 = 0, KIND_TF32 = 1, KIND_I8 = 2, KIND_F8F6F4 = 3 };
 
 // where a bounded wait gave up (status word 1, bits 31..24)
-enum { SITE_PRODUCER_EMPTY = 1, SITE_MMA_FULL = 2, SITE_MMA_TMEM_EMPTY = 3, SITE_EPI_TMEM_FULL = 4, SITE_COPY_TILE = 5 };
+enum { SITE_PRODUCER_EMPTY = 1, SITE_MMA_FULL = 2, SITE_MMA_TMEM_EMPTY = 3, SITE_EPI_TMEM_FULL = 4, SITE_COPY_TILE = 5, SITE_EPI_SCALES = 6 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 

@@ -392,6 +392,8 @@ const char* accb_version(void);
  *   "gemm.verbose"           0 | 1                    print the launch plan to stderr
  *   "gemm_fp8.kernel"        0 (choose) | 1 | 2       accb_gemm_fp8: 256 x 256 tiles by CTA pairs (1), tiles of 128 columns and 16 to 64 rows (2)
  *   "gemm_fp8.slices"        0 (choose) | 1 | 2 | 4 | 8   K slices of either
+ *   "gemm_fp8.test_drop_scales"  0 | 1                self-test: the last scales of a tile (or of a CTA's slice of K) are never
+ *                                                     signalled complete, with the same outcome as gemm.test_drop_commit
  *   "stream_kernels.pdl"     -1 (on) | 0 | 1          programmatic dependent launch of the reduce_mean, gather and range kernels
  *   "host_gemm.stage_chunks" 0 (16) | 1..256          row chunks of the staged host-pointer GEMM
  *   "reduce.rows_threads_per_output"  0 (choose) | 32 | 64 | 128 | 256   reduce_mean over contiguous segments

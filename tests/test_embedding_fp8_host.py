@@ -153,3 +153,10 @@ def test_bad_token_ids_are_attributed_to_the_launch_that_had_them():
     assert code == rt.ERR_INDEX and "4 token id(s)" in msg
     assert rt.decode_status(words, EMBED, 13) == (0, "") and rt.decode_status(words, GATHER, 12) == (0, "")
     assert rt.decode_status(words, ALL)[0] == rt.ERR_INDEX
+
+
+def test_a_wait_for_scales_is_named():
+    code, msg = rt.decode_status([0, (6 << 24) | 5, 8, 77, 2, 0, 0, 0])
+    assert code == rt.ERR_TIMEOUT and "epilogue waiting for scales, block 5, step 8" in msg
+    with rt.options(**{"gemm_fp8.test_drop_scales": 1}):
+        pass

@@ -412,3 +412,23 @@ def test_a_tied_table_trained_one_step():
     both = head.double().index_add(0, ids, dx.cpu().double() * dim ** 0.5)
     size = head.double().abs().index_add(0, ids, dx.cpu().double().abs() * dim ** 0.5)
     assert ((dw.cpu().double() - both).abs() <= tokens * 2.0 ** -24 * size).all()
+
+
+@pytest.mark.parametrize("ga,gb", [(1, 128), (1, 1)])
+@pytest.mark.parametrize("path,k,dropped", [("pair", 1152, "scales"), ("pair", 512, "scales"), ("pair4", 4096, "scales"), ("tile", 1152, "scales"),
+                                            ("tile8", 4096, "scales"), ("pair4", 4096, "commit"), ("tile8", 4096, "commit")])
+def test_scales_and_slices_that_never_arrive_are_reported(path, k, dropped, ga, gb):
+    # 9 blocks of K (8 a slice with four slices): the last slot of scales begins behind blocks whose sums are on their way
+    m, n = 300, 520
+    A, sa, B, sb = _operands(m, n, k, "e4m3", "e4m3", ga, gb, 13)
+    want, err = _gemm_want(A, sa, B, sb, ga, gb)
+    rt.synchronize()
+    drop = {"scales": "gemm_fp8.test_drop_scales", "commit": "gemm.test_drop_commit"}[dropped]
+    with rt.options(**PATHS[path], **{drop: 1, "gemm.wait_limit_us": 20000}):
+        C = torch.zeros(m, n, device="cuda")
+        rt.gemm_fp8(A.cuda(), B.cuda().t(), C, sa.cuda(), sb.cuda().t(), beta=0.0)
+        with pytest.raises(rt.AccbError) as e:
+            rt.synchronize()
+        assert e.value.code == rt.ERR_TIMEOUT and ("waiting for scales" if dropped == "scales" else "waiting for the accumulator") in str(e.value)
+    with rt.options(**PATHS[path]):
+        _check(_run(A, sa, B, sb, ga, gb, "f32"), want, err, path)
