@@ -64,7 +64,8 @@ struct DeviceState {
     std::mutex pool_mu;             // creation of the pool (calls on host pointers hold mu while they allocate from it)
     bool ready = false;
     int num_sms = 0;
-    int* status = nullptr;          // device, kStatusWords ints
+    int* status = nullptr;          // device, kStatusWords ints (and the pace counters behind them): launches on device pointers
+    int* host_status = nullptr;     // the same for the launches of calls on host pointers, which hold mu until they have read it
     int* status_host = nullptr;     // pinned mirror
     void* slot[kSlots] = {};        // staging: A/data, B/indices, C/output, bias, scales of A, scales of B
     size_t slot_bytes[kSlots] = {};
@@ -115,10 +116,11 @@ int device_state(DeviceState** out, int* dev_out)
             return fail(ACCB_ERR_CUDA, buf);
         }
         s.num_sms = prop.multiProcessorCount;
-        e = cudaMalloc(&s.status, (kStatusWords + kPaceSlots) * sizeof(int));
+        e = cudaMalloc(&s.status, 2 * (kStatusWords + kPaceSlots) * sizeof(int));
         if (e != cudaSuccess) return fail_cuda("cudaMalloc(status)", e);
-        e = cudaMemset(s.status, 0, (kStatusWords + kPaceSlots) * sizeof(int));
+        e = cudaMemset(s.status, 0, 2 * (kStatusWords + kPaceSlots) * sizeof(int));
         if (e != cudaSuccess) return fail_cuda("cudaMemset(status)", e);
+        s.host_status = s.status + kStatusWords + kPaceSlots;
         e = cudaMallocHost(&s.status_host, kStatusWords * sizeof(int));
         if (e != cudaSuccess) return fail_cuda("cudaMallocHost(status)", e);
         s.ready = true;
@@ -154,10 +156,10 @@ int ensure(void** buf, size_t* have, size_t need)
 }
 
 // Reads the status words back (synchronises `stream`) and turns them into an error code.
-//   what = COLLECT_GEMM / COLLECT_GATHER: a synchronous host-pointer call asks about its own launches only
-//          (launch id `id`); a failure an earlier device-pointer launch left behind stays recorded for
-//          accb_synchronize and does not become this call's result.
-//   what = COLLECT_ALL: accb_synchronize reports whatever is recorded.
+//   what = COLLECT_GEMM / COLLECT_GATHER / COLLECT_EMBED: a synchronous host-pointer call asks about its own launches
+//          (launch id `id`) in words of its own; what device-pointer launches have recorded or still record stays for
+//          accb_synchronize, neither becomes this call's result nor hides it.
+//   what = COLLECT_ALL: accb_synchronize reports whatever device-pointer launches have recorded.
 // What is reported is cleared.
 enum { COLLECT_ALL = 0, COLLECT_GEMM = 1, COLLECT_GATHER = 2, COLLECT_EMBED = 3 };
 
@@ -202,7 +204,8 @@ int decode_status(const int* w, int what, int id, bool* clear_gemm, bool* clear_
 
 int collect_status(DeviceState& s, cudaStream_t stream, int what = COLLECT_ALL, int id = 0)
 {
-    cudaError_t e = cudaMemcpyAsync(s.status_host, s.status, kStatusWords * sizeof(int), cudaMemcpyDeviceToHost, stream);
+    int* words = what == COLLECT_ALL ? s.status : s.host_status;
+    cudaError_t e = cudaMemcpyAsync(s.status_host, words, kStatusWords * sizeof(int), cudaMemcpyDeviceToHost, stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
     if (e != cudaSuccess) return fail_cuda("kernel execution", e);
     int w[kStatusWords];
@@ -211,15 +214,25 @@ int collect_status(DeviceState& s, cudaStream_t stream, int what = COLLECT_ALL, 
     std::string msg;
     const int rc = decode_status(w, what, id, &clear_gemm, &clear_gather, &clear_embed, &msg);
     if (rc == ACCB_OK) return ACCB_OK;
-    if (clear_gemm) e = cudaMemsetAsync(s.status + ST_GEMM_SITE, 0, 4 * sizeof(int), stream);      // words 1..4
+    if (clear_gemm) e = cudaMemsetAsync(words + ST_GEMM_SITE, 0, 4 * sizeof(int), stream);      // words 1..4
     if (clear_gather && e == cudaSuccess) {
-        e = cudaMemsetAsync(s.status + ST_GATHER_COUNT, 0, sizeof(int), stream);
-        if (e == cudaSuccess) e = cudaMemsetAsync(s.status + ST_GATHER_ID, 0, sizeof(int), stream);
+        e = cudaMemsetAsync(words + ST_GATHER_COUNT, 0, sizeof(int), stream);
+        if (e == cudaSuccess) e = cudaMemsetAsync(words + ST_GATHER_ID, 0, sizeof(int), stream);
     }
-    if (clear_embed && e == cudaSuccess) e = cudaMemsetAsync(s.status + ST_EMBED_COUNT, 0, 2 * sizeof(int), stream);   // words 6, 7
+    if (clear_embed && e == cudaSuccess) e = cudaMemsetAsync(words + ST_EMBED_COUNT, 0, 2 * sizeof(int), stream);   // words 6, 7
     if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
     if (e != cudaSuccess) return fail_cuda("cudaMemsetAsync(status)", e);
     return fail(rc, msg);
+}
+
+// The words that the launches of a host-pointer call on `stream` record in, cleared (a call that ended early may have left
+// something); the caller holds s.mu until it has collected them.
+int use_host_status(DeviceState& s, cudaStream_t stream, int** words)
+{
+    const cudaError_t e = cudaMemsetAsync(s.host_status, 0, kStatusWords * sizeof(int), stream);
+    if (e != cudaSuccess) return fail_cuda("cudaMemsetAsync(status)", e);
+    *words = s.host_status;
+    return ACCB_OK;
 }
 
 size_t type_bytes(int t)
@@ -449,6 +462,7 @@ int pipelined_host_gemm(DeviceState& s, GemmLaunch g, const void* a, const void*
         if (!s.pipe[i]) e = cudaStreamCreateWithFlags(&s.pipe[i], cudaStreamNonBlocking);
     if (e == cudaSuccess && !s.pipe_ready) e = cudaEventCreateWithFlags(&s.pipe_ready, cudaEventDisableTiming);
     if (e != cudaSuccess) return fail_cuda("creating the staging pipeline", e);
+    if (const int rc = use_host_status(s, s.pipe[0], &g.status); rc != ACCB_OK) return rc;      // before pipe_ready: ordered on both streams
 
     // 16 row chunks by default (the host_stage_chunks option overrides): the copy in of the first chunk and
     // the copy out of the last one are the part of the pipeline that nothing overlaps.  Measured on
@@ -574,6 +588,7 @@ static int gemm_entry(const char* fn, const accb_gemm_desc* desc, int64_t batch,
         const bool row_major_ac = d.a_stride[1] == 1 && d.c_stride[1] == 1 && d.a_stride[0] >= d.k && d.c_stride[0] >= d.n;
         if (batch == 1 && row_major_ac && d.m >= 4096 && d.k > 0 && bytes_a + bytes_c >= ((size_t)64 << 20))
             return pipelined_host_gemm(s, g, a, b, c, bias, ea, ec, bytes_b);
+        if ((rc = use_host_status(s, g.stream, &g.status)) != ACCB_OK) return rc;
         cudaError_t e = cudaSuccess;
         if (bytes_a) e = cudaMemcpyAsync(s.slot[0], a, bytes_a, cudaMemcpyHostToDevice, g.stream);
         if (e == cudaSuccess && bytes_b) e = cudaMemcpyAsync(s.slot[1], b, bytes_b, cudaMemcpyHostToDevice, g.stream);
@@ -855,10 +870,12 @@ int accb_gather_rank2(const void* data, int64_t d0, int64_t d1, const int64_t* i
     if ((rc = ensure(&s.slot[0], &s.slot_bytes[0], bytes_data)) != ACCB_OK) return rc;
     if ((rc = ensure(&s.slot[1], &s.slot_bytes[1], bytes_idx)) != ACCB_OK) return rc;
     if ((rc = ensure(&s.slot[2], &s.slot_bytes[2], bytes_out)) != ACCB_OK) return rc;
+    int* status = nullptr;
+    if ((rc = use_host_status(s, stream, &status)) != ACCB_OK) return rc;
     cudaError_t e = cudaMemcpyAsync(s.slot[0], data, bytes_data, cudaMemcpyHostToDevice, stream);
     if (e == cudaSuccess) e = cudaMemcpyAsync(s.slot[1], indices, bytes_idx, cudaMemcpyHostToDevice, stream);
     if (e != cudaSuccess) return fail_cuda("host to device copy", e);
-    int n = launch_gather(s.slot[0], d0, d1, (const int64_t*)s.slot[1], i0, i1, s.slot[2], axis, elem_bytes, s.status, launch_id, stream, &err);
+    int n = launch_gather(s.slot[0], d0, d1, (const int64_t*)s.slot[1], i0, i1, s.slot[2], axis, elem_bytes, status, launch_id, stream, &err);
     if (n < 0) return fail(n, std::string("accb_gather_rank2: ") + err);
     e = cudaMemcpyAsync(output, s.slot[2], bytes_out, cudaMemcpyDeviceToHost, stream);
     if (e != cudaSuccess) return fail_cuda("device to host copy", e);
@@ -917,6 +934,7 @@ static int embedding_entry(const char* fn, bool grad, const accb_embedding_desc*
     if ((rc = ensure(&s.slot[0], &s.slot_bytes[0], bytes_table)) != ACCB_OK) return rc;
     if ((rc = ensure(&s.slot[1], &s.slot_bytes[1], bytes_ids)) != ACCB_OK) return rc;
     if ((rc = ensure(&s.slot[2], &s.slot_bytes[2], bytes_rows)) != ACCB_OK) return rc;
+    if ((rc = use_host_status(s, l.stream, &l.status)) != ACCB_OK) return rc;
     // the written side goes to the device too where it is read or has gaps between its rows, whose bytes come back
     const bool gaps = grad ? d.table_stride != d.dim : d.rows_stride != d.dim;
     const bool table_in = bytes_table && (!grad || d.beta != 0.0f || gaps), rows_in = bytes_rows && (grad || gaps);
@@ -1071,6 +1089,7 @@ int accb_gemm_fp8(const accb_gemm_desc* desc, const accb_fp8_scales* scales, con
         if (!bytes[i]) continue;
         if ((rc = ensure(&s.slot[i], &s.slot_bytes[i], bytes[i])) != ACCB_OK) return rc;
     }
+    if ((rc = use_host_status(s, g.stream, &g.status)) != ACCB_OK) return rc;
     for (int i = 0; i < kSlots; ++i) {
         if (!bytes[i] || (i == 2 && d.beta == 0.0f && c_dense)) continue;
         const cudaError_t e = cudaMemcpyAsync(s.slot[i], host[i], bytes[i], cudaMemcpyHostToDevice, g.stream);
