@@ -155,6 +155,12 @@ constexpr int kMaxBins = 1 << kMaxDigitBits;
 constexpr int kSortCluster = 8;
 constexpr size_t kSortSmem = ((size_t)kSortWarps * kMaxBins + 2 * kMaxBins + kSortWarps) * 4;
 
+// An id outside the table is a mistake unless it is the padding id; a negative padding_id stands for none, so that no id equals it
+__device__ __forceinline__ bool bad_id(int64_t id, int vocab, int64_t padding_id)
+{
+    return (uint64_t)id >= (uint64_t)vocab && (id < 0 || id != padding_id);
+}
+
 struct SortParams {
     int n;
     int vocab;
@@ -214,7 +220,7 @@ __device__ void sort_tokens(const void* ids, int* keys0, int* tokens0, int* keys
         for (int i = begin + lane; i < end; i += 32) {
             if (pass == 0) {
                 const int64_t id = load_id(ids, i, p.id_bytes);
-                bad += !((uint64_t)id < (uint64_t)p.vocab) && id != p.padding_id;
+                bad += bad_id(id, p.vocab, p.padding_id);
             }
             atomicAdd(&hist[warp][(key_at(i) >> shift) & (bins - 1)], 1);
         }
@@ -607,9 +613,8 @@ few_tokens_kernel(const TR* __restrict__ rows, const void* __restrict__ ids, TT*
     }
     const int token = blockIdx.x / p.slabs, slab = blockIdx.x % p.slabs;
     const int64_t word = load_id(ids, token, sp.id_bytes);
-    const bool good = (uint64_t)word < (uint64_t)sp.vocab;
-    if (!good || word == sp.padding_id) {
-        if (!good && word != sp.padding_id && slab == 0 && threadIdx.x == 0) { atomicAdd(status + ST_EMBED_COUNT, 1); status[ST_EMBED_ID] = sp.launch_id; }
+    if ((uint64_t)word >= (uint64_t)sp.vocab || word == sp.padding_id) {
+        if (bad_id(word, sp.vocab, sp.padding_id) && slab == 0 && threadIdx.x == 0) { atomicAdd(status + ST_EMBED_COUNT, 1); status[ST_EMBED_ID] = sp.launch_id; }
         return;
     }
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -746,7 +751,7 @@ int launch_grad(const EmbeddingLaunch& l, const void* rows, void* table, const c
     const int64_t n = d.tokens;
     const bool vec = vector_rows<TT, TR>(d, table, rows), clear = d.beta != 1.0f;
     SortParams s;
-    s.n = (int)n; s.vocab = (int)d.vocab; s.padding_id = d.padding_id < 0 ? INT64_MIN : d.padding_id;   // (an id of -1 is out of range, not padding)
+    s.n = (int)n; s.vocab = (int)d.vocab; s.padding_id = d.padding_id;
     s.id_bytes = d.id_bytes;
     int bits = 1;
     while (((int64_t)1 << bits) <= d.vocab) ++bits;          // keys 0 .. vocab

@@ -277,3 +277,16 @@ def test_offsets_beyond_32_bits():
     rt.synchronize()
     assert (out[0] == 3).all() and (out[1] == 0).all() and (table[vocab - 1] == 9).all() and (table[0] == 0).all()
     assert (table[vocab - 2] == 0).all()
+
+
+@pytest.mark.parametrize("tokens", [4, 3000])                             # few tokens, and sorted
+@pytest.mark.parametrize("padding", [None, 3])
+def test_every_negative_id_is_reported(tokens, padding):
+    ids = torch.full((tokens,), 2)
+    ids[0], ids[1], ids[2] = -2 ** 63, -1, 3
+    got = torch.empty(10, 8, device="cuda")
+    rt.synchronize()
+    rt.embedding_grad(torch.ones(tokens, 8, device="cuda"), ids.cuda(), got, padding_id=padding)
+    with pytest.raises(rt.AccbError, match=r"embedding: 2 token id"):
+        rt.synchronize()
+    assert (got[2] == tokens - 3).all() and (got[3] == (0 if padding else 1)).all() and got.sum() == 8 * (tokens - (3 if padding else 2))
