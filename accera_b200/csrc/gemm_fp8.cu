@@ -1099,7 +1099,8 @@ int launch_gemm_fp8(const GemmFp8Launch& g0, const char** err)
     const int b_dir = contiguous_direction(d.n, d.k, d.b_stride[1], d.b_stride[0]);
     if (d.k < 1 || a_dir < 0 || b_dir < 0 || !encode_tiled_fn()) return 0;
 
-    // Operands as `lines` runs of `width` bytes, `pitch` bytes apart.  TMA wants 16-byte aligned runs: others are copied.
+    // Operands as `lines` runs of `width` bytes, `pitch` bytes apart.  TMA wants 16-byte aligned runs that do not overlap: others
+    // are copied.
     struct Operand { const void* base; int64_t lines, width, pitch; } op[2] = {
         { g.a, a_dir ? d.k : d.m, a_dir ? d.m : d.k, a_dir ? d.a_stride[1] : d.a_stride[0] },
         { g.b, b_dir ? d.k : d.n, b_dir ? d.n : d.k, b_dir ? d.b_stride[0] : d.b_stride[1] } };
@@ -1109,7 +1110,7 @@ int launch_gemm_fp8(const GemmFp8Launch& g0, const char** err)
     for (int i = 0; i < 2; ++i) {
         Operand& o = op[i];
         if (o.lines == 1) o.pitch = (o.width + 15) / 16 * 16;            // never followed
-        if (o.pitch % 16 == 0 && (reinterpret_cast<uintptr_t>(o.base) & 15) == 0) continue;
+        if (o.pitch % 16 == 0 && o.pitch >= o.width && (reinterpret_cast<uintptr_t>(o.base) & 15) == 0) continue;
         const int64_t pitch = (o.width + 15) / 16 * 16;
         tmp[i] = temp_alloc(g.device, (size_t)(pitch * o.lines), g.stream);
         if (!tmp[i]) { release(); *err = "no device memory for an aligned copy of an operand"; return ACCB_ERR_CUDA; }

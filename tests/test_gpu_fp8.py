@@ -432,3 +432,21 @@ def test_scales_and_slices_that_never_arrive_are_reported(path, k, dropped, ga, 
         assert e.value.code == rt.ERR_TIMEOUT and ("waiting for scales" if dropped == "scales" else "waiting for the accumulator") in str(e.value)
     with rt.options(**PATHS[path]):
         _check(_run(A, sa, B, sb, ga, gb, "f32"), want, err, path)
+
+
+@pytest.mark.parametrize("path", ["pair", "pair4", "tile", "auto"])
+@pytest.mark.parametrize("step", [16, 48, 1, 7])
+def test_gemm_operands_whose_rows_overlap(path, step):
+    # windows of a longer signal: rows of A 16, 48, 1 or 7 bytes apart; the same for the columns of B
+    m, n, k = 90, 150, 520
+    g = torch.Generator().manual_seed(14)
+    signal = [(torch.randn(max(m, n) * step + k, generator=g) * 40).to(torch.float8_e4m3fn).cuda() for _ in range(2)]
+    A, B = signal[0].as_strided((m, k), (step, 1)), signal[1].as_strided((n, k), (step, 1))
+    _, sa, _, sb = _operands(m, n, k, "e4m3", "e4m3", 1, 128, 15)
+    Ac, Bc = A.cpu().contiguous(), B.cpu().contiguous()
+    want, err = _gemm_want(Ac, sa, Bc, sb, 1, 128)
+    C = torch.full((m, n), float("nan"), device="cuda")
+    with rt.options(**PATHS[path]):
+        rt.gemm_fp8(A, B.t(), C, sa.cuda(), sb.cuda().t(), beta=0.0)
+    rt.synchronize()
+    _check(C.cpu(), want, err, (path, step))
