@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
+import sys
 from typing import Optional
 
 import numpy as np
@@ -227,7 +228,8 @@ def release_workspace() -> None:
 # ---------------------------------------------------------------------------
 
 def _is_torch(x) -> bool:
-    return type(x).__module__.split(".")[0] == "torch"
+    """A torch tensor, of a subclass from another package too; does not import torch for callers that have not."""
+    return isinstance(x, getattr(sys.modules.get("torch"), "Tensor", ()))
 
 
 def _describe(x, kind: Optional[str] = None):

@@ -1,5 +1,8 @@
 """What the token table and 8-bit floating point entry points refuse, checked without a GPU."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -160,3 +163,27 @@ def test_a_wait_for_scales_is_named():
     assert code == rt.ERR_TIMEOUT and "epilogue waiting for scales, block 5, step 8" in msg
     with rt.options(**{"gemm_fp8.test_drop_scales": 1}):
         pass
+
+
+_SUBCLASS = """
+import torch
+from accera_b200 import runtime as rt
+
+class Marked(torch.Tensor):
+    pass
+
+make = lambda *shape: torch.zeros(*shape).as_subclass(Marked)
+{first}
+"""
+
+
+@pytest.mark.parametrize("first,text", [
+    ("rt.embedding(make(9), make(3), make(3, 8))", "ids: unsupported tensor dtype"),
+    ("rt.quantize_fp8(make(4, 8), make(4, 8), make(4, 1))", "q: unsupported tensor dtype"),
+    ("rt.gemm_fp8(make(4, 8), make(8, 4), make(4, 4), make(4, 1), make(1, 1))", "A: unsupported tensor dtype"),
+    ("rt.gemm(make(4, 8), make(7, 4), make(4, 4))", "shape mismatch"),
+])
+def test_a_tensor_subclass_may_be_the_first_argument_of_a_process(first, text):
+    r = subprocess.run([sys.executable, "-c", _SUBCLASS.format(first=first)], capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode != 0 and text in r.stderr, r.stderr
