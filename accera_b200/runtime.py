@@ -583,9 +583,9 @@ def _load_torch() -> None:
     _torch_tensor = (torch.Tensor,)
 
 
-def _operand(name: str, x, accepted, kind: Optional[str] = None):
+def _operand(name: str, x, accepted, kind: Optional[str] = None, written: bool = False):
     """-> (pointer, element type code, shape, element strides, device index or -1 for host memory) of an array whose type
-    is one of `accepted` (type codes).  bf16 and 8-bit floating point numpy arrays are bit patterns (uint16, uint8) that `kind` names."""
+    is one of `accepted` (type codes); `written`: a result, so not a read-only array.  bf16 and 8-bit floating point numpy arrays are bit patterns (uint16, uint8) that `kind` names."""
     if isinstance(x, _torch_tensor):
         code = _torch_codes.get(x.dtype, -1)
         if code not in accepted:
@@ -606,10 +606,12 @@ def _operand(name: str, x, accepted, kind: Optional[str] = None):
             raise TypeError(f"{name}: unsupported element type {x.dtype}")
         if any(st % x.itemsize for st in x.strides):
             raise ValueError(f"{name}: strides must be whole elements")
+        if written and not x.flags.writeable:
+            raise ValueError(f"{name}: the array is read-only")
         return x.ctypes.data, code, x.shape, tuple(st // x.itemsize for st in x.strides), -1
     if not _torch_tensor and _is_torch(x):
         _load_torch()
-        return _operand(name, x, accepted, kind)
+        return _operand(name, x, accepted, kind, written)
     raise TypeError(f"{name}: expected a numpy array or a torch tensor")
 
 
@@ -649,9 +651,9 @@ def _row_stride(name, rows, cols, s0, s1) -> int:
 
 
 def _embedding_call(entry, table, ids, rows, scale, beta, padding_id, table_kind, rows_kind) -> None:
-    pt, tt, sht, stt, dt = _operand("table", table, _FLOATS, table_kind)
+    pt, tt, sht, stt, dt = _operand("table", table, _FLOATS, table_kind, entry == 1)
     pi, ti, shi, sti, di = _operand("ids", ids, _IDS)
-    pr, tr, shr, str_, dr = _operand("rows", rows, _FLOATS, rows_kind)
+    pr, tr, shr, str_, dr = _operand("rows", rows, _FLOATS, rows_kind, entry == 0)
     if len(sht) != 2:
         raise ValueError("table must be rank 2")
     vocab, dim = sht
@@ -725,8 +727,8 @@ def quantize_fp8(x, q, scales, *, kind: Optional[str] = None, q_kind: Optional[s
     transposed result with groups down the columns of x: the form a weight-gradient product needs.
     """
     px, tx, shx, stx, dx = _operand("x", x, _FLOATS, kind)
-    pq, tq, shq, stq, dq = _operand("q", q, _FP8, q_kind)
-    ps, _, shs, sts, ds = _operand("scales", scales, _ONLY_F32)
+    pq, tq, shq, stq, dq = _operand("q", q, _FP8, q_kind, True)
+    ps, _, shs, sts, ds = _operand("scales", scales, _ONLY_F32, None, True)
     if len(shx) != 2 or shq != shx or len(shs) != 2:
         raise ValueError(f"shape mismatch: x{tuple(shx)} q{tuple(shq)} scales{tuple(shs)}")
     rows, cols = shx
@@ -754,7 +756,7 @@ def gemm_fp8(A, B, C, a_scales, b_scales, *, bias=None, alpha: float = 1.0, beta
     """
     pa, ta, sha, sta, da = _operand("A", A, _FP8, a_kind)
     pb, tb, shb, stb, db = _operand("B", B, _FP8, b_kind)
-    pc, tc, shc, stc, dc = _operand("C", C, _FLOATS, out_kind)
+    pc, tc, shc, stc, dc = _operand("C", C, _FLOATS, out_kind, True)
     psa, _, shsa, stsa, dsa = _operand("a_scales", a_scales, _ONLY_F32)
     psb, _, shsb, stsb, dsb = _operand("b_scales", b_scales, _ONLY_F32)
     if not len(sha) == len(shb) == len(shc) == len(shsa) == len(shsb) == 2:

@@ -187,3 +187,23 @@ def test_a_tensor_subclass_may_be_the_first_argument_of_a_process(first, text):
     r = subprocess.run([sys.executable, "-c", _SUBCLASS.format(first=first)], capture_output=True, text=True, timeout=300,
                        cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert r.returncode != 0 and text in r.stderr, r.stderr
+
+
+def test_results_are_not_written_to_read_only_arrays():
+    f, q = lambda *shape: np.zeros(shape, np.float32), lambda *shape: np.zeros(shape, np.uint8)
+    ids = np.zeros(3, np.int64)
+
+    def fixed(x):
+        x.flags.writeable = False
+        return x
+
+    kinds = dict(a_kind="float8_e4m3", b_kind="float8_e4m3")
+    for call, name in [(lambda: rt.embedding(f(9, 8), ids, fixed(f(3, 8))), "rows"), (lambda: rt.embedding_grad(f(3, 8), ids, fixed(f(9, 8))), "table"),
+                       (lambda: rt.quantize_fp8(f(4, 8), fixed(q(4, 8)), f(4, 1), q_kind="float8_e4m3"), "q"),
+                       (lambda: rt.quantize_fp8(f(4, 8), q(4, 8), fixed(f(4, 1)), q_kind="float8_e4m3"), "scales"),
+                       (lambda: rt.gemm_fp8(q(4, 8), q(8, 6), fixed(f(4, 6)), f(4, 1), f(1, 1), **kinds), "C")]:
+        with pytest.raises(ValueError, match=f"{name}: the array is read-only"):
+            call()
+    if not rt.device_count():                                              # what is only read may be read-only
+        with pytest.raises(rt.AccbError):
+            rt.embedding(fixed(f(9, 8)), fixed(ids.copy()), f(3, 8))
