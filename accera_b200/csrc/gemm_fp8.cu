@@ -1116,6 +1116,7 @@ int launch_gemm_fp8(const GemmFp8Launch& g0, const char** err)
         if (!tmp[i]) { release(); *err = "no device memory for an aligned copy of an operand"; return ACCB_ERR_CUDA; }
         const int rc = launch_repack_rows(o.base, o.pitch, o.lines, o.width, 1, tmp[i], pitch, o.lines, g.stream, err);
         if (rc < 0) { release(); return rc; }
+        note_launches(rc);
         launches += rc;
         o.base = tmp[i];
         o.pitch = pitch;

@@ -451,3 +451,15 @@ def test_gemm_operands_whose_rows_overlap(path, step):
         rt.gemm_fp8(A, B.t(), C, sa.cuda(), sb.cuda().t(), beta=0.0)
     rt.synchronize()
     _check(C.cpu(), want, err, (path, step))
+
+
+def test_aligned_copies_count_as_launches():
+    m, n, k = 40, 512, 1000                                           # rows of 1000 bytes: both operands are copied
+    A, sa, B, sb = [t.cuda() for t in _operands(m, n, k, "e4m3", "e4m3", 1, 128, 23)]
+    C = torch.empty(m, n, device="cuda")
+    for path, launches in (("tile2", 3), ("pair", 3), ("pair4", 4)):
+        with rt.options(**PATHS[path]):
+            before = rt.launch_count()
+            rt.gemm_fp8(A, B.t(), C, sa, sb.t(), beta=0.0)
+            assert rt.launch_count() - before == launches, path
+    rt.synchronize()
