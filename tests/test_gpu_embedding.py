@@ -290,3 +290,27 @@ def test_every_negative_id_is_reported(tokens, padding):
     with pytest.raises(rt.AccbError, match=r"embedding: 2 token id"):
         rt.synchronize()
     assert (got[2] == tokens - 3).all() and (got[3] == (0 if padding else 1)).all() and got.sum() == 8 * (tokens - (3 if padding else 2))
+
+
+@pytest.mark.parametrize("tg,tt", [("f32", "f32"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("tokens,vocab,dim", [(4000, 70, 1001), (30000, 900, 33), (29000, 5000, 136), (10000, 300, 2056), (3000, 300, 2056)])
+@pytest.mark.parametrize("kind", ["runs", "zipf"])
+def test_sorted_gradients_of_many_blocks(kind, tokens, vocab, dim, tg, tt):
+    # blocks of 32 tokens and a slab of columns, beyond six an SM but for the last size: rows of whole vectors and others, long and
+    # short words
+    ids = _ids(kind, tokens, vocab, 8)
+    g = torch.randn(tokens, dim, generator=torch.Generator().manual_seed(dim)).to(TYPES[tg])
+    old = torch.randn(vocab, dim, generator=torch.Generator().manual_seed(9)).to(TYPES[tt])
+    want, err = _grad_want(g, ids, old, 0.5, 1.0, 1, vocab)
+    got = old.cuda()
+    rt.embedding_grad(g.cuda(), ids.cuda(), got, scale=0.5, beta=1.0, padding_id=1)
+    rt.synchronize()
+    _check_grad(got.cpu(), want, err, (kind, tg, tt))
+    want, err = _grad_want(g, ids, None, 0.5, 0.0, None, vocab)
+    got = torch.full((vocab, dim), float("nan"), device="cuda", dtype=TYPES[tt])
+    again = torch.full((vocab, dim), 3.0, device="cuda", dtype=TYPES[tt])
+    rt.embedding_grad(g.cuda(), ids.cuda(), got, scale=0.5)
+    rt.embedding_grad(g.cuda(), ids.int().cuda(), again, scale=0.5)
+    rt.synchronize()
+    _check_grad(got.cpu(), want, err, (kind, tg, tt))
+    assert torch.equal(got, again)

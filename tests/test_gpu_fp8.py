@@ -463,3 +463,174 @@ def test_aligned_copies_count_as_launches():
             rt.gemm_fp8(A, B.t(), C, sa, sb.t(), beta=0.0)
             assert rt.launch_count() - before == launches, path
     rt.synchronize()
+
+
+def _check_16(got, want, err, what):
+    """_check, for results some of which fp16 cannot hold: from 65520 (its largest value and half a step) on they round to infinity;
+    within the bound of that border either answer is right."""
+    if got.dtype != torch.float16:
+        return _check(got, want, err, what)
+    over = want.abs() - err >= 65520
+    near = ~over & (want.abs() + err >= 65520)
+    assert torch.equal(got[over].double(), torch.sign(want[over]) * float("inf")), what
+    _check(torch.where(over | near, torch.zeros_like(got), got), torch.where(over | near, torch.zeros_like(want), want), err, what)
+
+
+# (200, 264): rows of C that are whole vectors in every type; (130, 203): not; (512, 512): whole tiles, stored without an epilogue's branches
+@pytest.mark.parametrize("alpha,beta,relu,use_bias", [(1.0, 0.0, False, False), (0.5, 0.0, True, True), (-2.0, 0.25, False, True), (1.0, 1.0, True, True)])
+@pytest.mark.parametrize("c", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("ga,gb", [(1, 1), (128, 1), (128, 128), (1, 128)])
+@pytest.mark.parametrize("path", ["pair", "pair4", "tile2"])
+@pytest.mark.parametrize("m,n,k", [(200, 264, 768), (130, 203, 700), (512, 512, 640)])
+def test_gemm_epilogue_with_every_scale_layout(alpha, beta, relu, use_bias, c, ga, gb, path, m, n, k):
+    A, sa, B, sb = _operands(m, n, k, "e4m3", "e4m3", ga, gb, 16)
+    g = torch.Generator().manual_seed(17)
+    sb *= 0.0005                                                       # nearly all inside fp16's range
+    old = (torch.randn(m, n, generator=g) * 100).to(TYPES[c])
+    bias = torch.randn(n, generator=g) * 100 if use_bias else None
+    want, err = _gemm_want(A, sa, B, sb, ga, gb, old, alpha, beta, bias, relu)
+    with rt.options(**PATHS[path]):
+        got = _run(A, sa, B, sb, ga, gb, c, old=old, alpha=alpha, beta=beta, relu=relu, bias=bias)
+    _check_16(got, want, err, "epilogue")
+
+
+@pytest.mark.parametrize("a,b", [("e4m3", "e4m3"), ("e5m2", "e4m3"), ("e4m3", "e5m2")])
+@pytest.mark.parametrize("c", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("layout", ["tn", "tt", "nn", "nt"])
+@pytest.mark.parametrize("ga,gb", [(1, 1), (128, 1)])
+@pytest.mark.parametrize("path,m,n,k", [("pair", 272, 400, 528), ("pair4", 272, 400, 1040), ("tile", 40, 272, 528)])
+def test_gemm_types_and_layouts_with_a_scale_per_column(a, b, c, layout, ga, gb, path, m, n, k):
+    A, sa, B, sb = _operands(m, n, k, a, b, ga, gb, 18)
+    sb *= 0.0005
+    want, err = _gemm_want(A, sa, B, sb, ga, gb)
+    with rt.options(**PATHS[path]):
+        got = _run(A, sa, B, sb, ga, gb, c, layout, compute="tensor")
+    _check_16(got, want, err, (a, b, c, layout))
+
+
+@pytest.mark.parametrize("c", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("beta", [0.0, 1.0])
+@pytest.mark.parametrize("gb", [1, 128])
+@pytest.mark.parametrize("path,m,n,k", [("pair", 200, 300, 384), ("pair4", 200, 300, 512), ("pair", 33, 257, 130), ("tile2", 33, 257, 300)])
+def test_gemm_result_strides_of_every_type_leave_the_rest_alone(c, beta, gb, path, m, n, k):
+    A, sa, B, sb = _operands(m, n, k, "e4m3", "e4m3", 1, gb, 19)
+    sb *= 0.0005
+    old = torch.full((m, n), 7.0).to(TYPES[c])
+    want, err = _gemm_want(A, sa, B, sb, 1, gb, old, 1.0, beta)
+    full = lambda *shape: torch.full(shape, 7.0, device="cuda", dtype=TYPES[c])
+    for make in (lambda: full(m, n + 5)[:, 2:n + 2], lambda: full(n + 3, m + 1)[1:n + 1, :m].t(), lambda: full(m, 2 * n)[:, ::2], lambda: full(m, n + 16 - n % 8)[:, 8:n + 8]):
+        C = make()
+        base = C._base
+        with rt.options(**PATHS[path]):
+            rt.gemm_fp8(A.cuda(), B.cuda().t(), C, sa.cuda(), sb.cuda().t(), beta=beta)
+        rt.synchronize()
+        _check_16(C.cpu(), want, err, tuple(C.stride()))
+        left = base.clone()
+        left.as_strided(C.shape, C.stride(), C.storage_offset()).fill_(7.0)
+        assert (left == 7).all()
+
+
+@pytest.mark.parametrize("c", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("ga,gb", [(1, 1), (128, 128)])
+@pytest.mark.parametrize("max_ctas", [0, 2, 7])
+def test_gemm_over_several_groups_of_row_tiles(c, ga, gb, max_ctas):
+    # 11 row tiles of 256: a whole group of eight and a part of one; with two or six CTAs every pair takes many tiles, the ring
+    # of scales and both accumulators running on from one to the next
+    m, n, k = 2700, 600, 1152
+    A, sa, B, sb = _operands(m, n, k, "e4m3", "e4m3", ga, gb, 20)
+    sb *= 0.0005
+    want, err = _gemm_want(A, sa, B, sb, ga, gb)
+    with rt.options(**PATHS["pair"]):
+        got = _run(A, sa, B, sb, ga, gb, c, max_ctas=max_ctas)
+    _check_16(got, want, err, (ga, gb, max_ctas))
+
+
+def _with_temporaries(kind):
+    """-> (options, m, n, k, offset of A's rows): calls that take aligned copies, sums of K slices, or both from the library's pool"""
+    return {"copy": (PATHS["pair"], 300, 512, 1000, 3), "slices": (PATHS["pair4"], 300, 512, 2048, 0), "both": (PATHS["pair4"], 300, 512, 2000, 3),
+            "copy, tile": (PATHS["tile2"], 40, 512, 1000, 3)}[kind]
+
+
+@pytest.mark.parametrize("kind", ["copy", "slices", "both", "copy, tile"])
+@pytest.mark.parametrize("gb", [1, 128])
+def test_gemm_temporaries_are_not_shared_by_streams_and_graphs(kind, gb):
+    path, m, n, k, lead = _with_temporaries(kind)
+    data, want = [], []
+    for seed in (21, 22):                                              # different inputs: a shared temporary would show
+        A, sa, B, sb = _operands(m, n, k, "e4m3", "e4m3", 1, gb, seed)
+        wide = torch.zeros(m, k + 7).to(torch.float8_e4m3fn)
+        wide[:, lead:lead + k] = A
+        data.append([wide.cuda()[:, lead:lead + k] if lead else A.cuda(), B.cuda().t(), sa.cuda(), sb.cuda().t()])
+        want.append(_gemm_want(A, sa, B, sb, 1, gb))
+
+    def call(i, C):
+        A, B, sa, sb = data[i]
+        rt.gemm_fp8(A, B, C, sa, sb, beta=0.0)
+
+    with rt.options(**path):
+        first = [torch.empty(m, n, device="cuda") for _ in range(2)]
+        for i in range(2):
+            call(i, first[i])
+        rt.synchronize()
+        for i in range(2):
+            _check_16(first[i].cpu(), *want[i], kind)
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        got = [torch.empty(m, n, device="cuda") for _ in range(2)]
+        torch.cuda.synchronize()
+        for _ in range(30):
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    call(i, got[i])
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], first[0]) and torch.equal(got[1], first[1])
+        graphs = []
+        for i in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                for _ in range(2):                                     # twice: a freed temporary used again inside the graph
+                    call(i, got[i])
+            graphs.append(graph)
+        other = [torch.empty(m, n, device="cuda") for _ in range(2)]
+        for g in got:
+            g.fill_(5.0)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    graphs[i].replay()
+                call(i, other[i])                                      # and eager calls beside the replays, on a third stream
+        torch.cuda.synchronize()
+        rt.synchronize()
+        for i in range(2):
+            assert torch.equal(got[i], first[i]) and torch.equal(other[i], first[i])
+
+
+@pytest.mark.parametrize("block", [1, 128])
+@pytest.mark.parametrize("across", [False, True])
+@pytest.mark.parametrize("src", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("to", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("m,k", [(264, 392), (131, 259), (2, 128)])
+def test_quantisation_of_infinities_nan_and_subnormals(block, across, src, to, m, k):
+    x = _values(m, k, m + k).to(TYPES[src])
+    inf, nan = float("inf"), float("nan")
+    for i, v in enumerate([inf, -inf, nan, -nan]):                     # in every word, half and lane; whole vectors of them; a group's largest
+        x[(7 * i) % m, (11 * i) % k] = v
+        x[(7 * i + 1) % m, (11 * i + 1) % k] = v
+        x[m - 1, (k - 1 - 3 * i) % k] = v
+    if m > 64:
+        x[40, 32:64] = inf
+        x[50, :128] = nan                                              # a group of nothing finite
+        x[51, :] = 0.0
+        x[52, :] = torch.finfo(TYPES[src]).smallest_normal * torch.finfo(TYPES[src]).eps * 3     # subnormal
+        x[53, 5] = torch.finfo(TYPES[src]).max
+        x[64:96, 130] = nan
+    if m > 256:
+        x[128:256, 128:256] = torch.tensor([inf, nan]).repeat(128, 64).to(TYPES[src])            # a tile of nothing finite
+    want = _quantize_want(x.double().numpy(), to, block)
+    xd = x.t().contiguous().cuda().t() if across else x.cuda()
+    q = torch.zeros(m, k, dtype=TYPES[to], device="cuda")
+    s = torch.zeros(_up(m, block), _up(k, 128), device="cuda")
+    rt.quantize_fp8(xd, q, s)
+    rt.synchronize()
+    assert _same(s.cpu().double().numpy(), want[1])
+    assert _same(q.cpu().double().numpy(), want[0])
