@@ -56,9 +56,9 @@ struct Options {
     int host_stage_chunks = 0;       // row chunks of the staged host-pointer GEMM (default 16)
     int reduce_rows_tpr = 0;         // reduce_mean over contiguous segments: threads per output (32, 64, 128 or 256)
     int gemm_fp8_kernel = 0;         // 8-bit GEMM: 1 = pair kernel, 2 = tile kernel
-    int gemm_fp8_slices = 0;         // tile kernel: K slices (1, 2, 4 or 8)
+    int gemm_fp8_slices = 0;         // 8-bit GEMM: K slices of either kernel (1, 2, 4 or 8)
     int gemm_fp8_test_drop_scales = 0;   // self-test: the arrival of a tile's (or slice's) last scales is left out
-    int stream_pdl = -1;             // programmatic dependent launch of the reduce / gather / range kernels: 0 off, 1 on
+    int stream_pdl = -1;             // programmatic dependent launch of the kernels that launch_pdl starts: 0 off, 1 on
 };
 Options& options();
 

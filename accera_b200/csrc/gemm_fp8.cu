@@ -10,13 +10,17 @@
 // Two kernels:
 //   pair   256 x 256 tiles by CTA pairs (cta_group::2), persistent: every SM multiplies 128 x 256 x 128 a block, in
 //          512 cycles at the nominal 8-bit rate.  Eight epilogue warps hold the sums, 128 fp32 a thread; while a warp adds
-//          32 columns the next 32 are on their way from TMEM.  8192^3, e4m3 to bf16: 550 us (2.0 PFLOP/s); the same loads and
-//          MMAs without the additions take 397 us, so the loop is bound by the round trip of a TMEM buffer (MMAs done -
+//          32 columns the next 32 are on their way from TMEM.  8192^3, e4m3 to bf16: 630 us call after call on three sets of
+//          inputs (1.75 PFLOP/s under the power limit), 550 to 590 in short runs; the same loads and MMAs without the
+//          additions take 397 us in short runs, so the loop is bound by the round trip of a TMEM buffer (MMAs done -
 //          read by both CTAs' warps - MMA issued again), of which only two fit TMEM at this width.  Narrower tiles with
-//          three or four buffers (160, 128 columns) were measured slower, 650 and 700 us: their operands alone take 500 and 540.
+//          three or four buffers (160, 128 columns) were measured slower, 650 and 700 us in short runs: their operands alone
+//          take 500 and 540.  With a scale per column 4096 x 8192 x 16384 takes 840 to 860 us (each product costs the
+//          epilogue warps two instructions instead of one).  The 168 registers a thread do not hold everything: 52 to 92 bytes a
+//          thread are spilled, 296 to 424 with a scale per column.
 //          Problems with few tiles cut K into slices, whose fp32 sums gemm_splitk.cu adds in slice order.
-//   tile   128 x BN tiles by single CTAs for up to 64 rows of C: columns of C (weights) on the 128 TMEM
-//          lanes, rows of C (tokens) on BN = 16 .. 64 accumulator columns, K cut into up to eight slices
+//   tile   128 x BN tiles by single CTAs, for few rows of C, or few tiles: columns of C (weights) on the 128 TMEM
+//          lanes, 16 to 64 rows of C (tokens) on BN = 16, 32 or 64 accumulator columns, K cut into up to eight slices
 //          that a cluster multiplies side by side and adds, slice by slice, through distributed shared memory.
 // Scales reach shared memory by cp.async up to sixteen blocks ahead, four blocks of a row in 16 bytes where they lie side by
 // side (4 bytes at a time the copies themselves bound the pair kernel with a scale per column).
@@ -675,7 +679,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             TC* dst = SPLIT ? C + slice * p.slice_stride : C;
             if (p.plain && row0 + 32 <= p.m && col0 + 128 <= p.n) {
                 // Nothing but the sums, all inside the matrix.  This code runs once a tile and is not in the instruction cache then,
-                // so the common case is kept short and without branches (8192^3 with a scale per column: 897 -> 833 us).
+                // so the common case is kept short and without branches (7 % of the time of 8192^3 with a scale per column).
                 constexpr int V = 16 / (int)sizeof(TC);
                 const int r0 = lane >> 3, slot = lane & 7;
                 uint8_t* out = reinterpret_cast<uint8_t*>(dst + (row0 + r0) * p.cs0 + col0 + slot * V);
@@ -1142,6 +1146,7 @@ int launch_gemm_fp8(const GemmFp8Launch& g0, const char** err)
 
     // Which kernel, and how many slices of K, by estimated microseconds, fitted to measured launches (graph replays).
     //   pair   a round of tiles takes 0.55 a block of K and 6 at its ends; slices add a second pass: 6, and its bytes at 4 TB/s
+    //          (fitted with one scale per 128 columns; a scale per column takes about 0.95 a block, which the choice does not know)
     //   tile   a wave of CTAs (two an SM) takes 0.6, 0.7, 0.9 a block for 16, 32, 64 rows, two thirds of it with one CTA an SM;
     //          4 at its ends and 1, 2, 3 more for the sum over a cluster, which only pays within one wave
     // For example 64 x 4096 x 4096: tile with 8 slices 10.4, pair at best 19; 256 x 4096 x 4096: 19 and 20.6; 128 x 32000 x 4096: 62 and 49.

@@ -100,7 +100,9 @@ template <typename T> __device__ __forceinline__ float scaled(const Vec16<T>& w,
 // Groups along the rows of x.  TILE = false: a group is 128 neighbours of a row, taken by 128 * sizeof(T) / 16 threads
 // with one 16-byte load each.  TILE = true: a block takes one square tile.  A group's last lane to know its maximum is one
 // warp reduction away (redux.sync), so the loads in flight come from the many warps that fit an SM.  8192 x 8192 bf16 to e4m3:
-// rows 42 us, tiles 35 us; the bytes alone take 31 us.
+// rows 42 us, tiles 35 us; the bytes alone take 31 us.  fp32 to e4m3: rows 69 us, tiles 150 us (51 us); the 16 vectors a thread
+// of an fp32 tile do not fit its 64 registers (924 bytes are spilled), nor do all of the rows' in 32 (68 to 80 bytes).
+// Rows that are not whole vectors go by single elements: 16383 x 8191 bf16 197 us where 16384 x 8192 takes 81.
 constexpr int kRowThreads = 256;
 
 template <typename T, bool E5M2, bool TILE, bool VEC>
@@ -200,7 +202,7 @@ quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __
 // x contiguous along its rows' index (a transposed view): a block takes 128 columns of the view (which lie a pitch apart in
 // memory) times a strip of its rows (contiguous), 64 rows or, for square tiles, 128.  A thread loads 16 bytes (E
 // rows) of four neighbouring columns, so that it can store four bytes of a result row at a time to shared
-// memory, from where rows of 128 bytes leave.  16384 x 8192 bf16 to e5m2: 85 us (4.8 TB/s); the bytes alone take 62 us.
+// memory, from where rows of 128 bytes leave.  16384 x 8192 bf16 to e5m2: 85 us (4.8 TB/s); the bytes alone take 62 us.  Unaligned, 16383 x 8191: 192 us by single elements.
 template <typename T, bool E5M2, bool TILE, bool VEC>
 __global__ void __launch_bounds__(256, TILE ? 4 : 6)
 quantize_across_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales, const Params p, int64_t row_blocks,

@@ -9,8 +9,8 @@
     python -m accera_b200.profile_cases reduce_cols [--rows 4096 --cols 8192]              (mean over the first axis)
     python -m accera_b200.profile_cases gather_elem [--table-rows 4096 --cols 32000 --indices 16384]   (gather along axis 1)
     python -m accera_b200.profile_cases gemm_fp8 [--m --n --k] [--column-scales]           (e4m3, one scale per 128 along K)
-    python -m accera_b200.profile_cases quantize_fp8 [--rows 8192 --cols 8192] [--across]
-    python -m accera_b200.profile_cases embedding | embedding_grad [--table-rows 32000 --cols 4096 --indices 16384]
+    python -m accera_b200.profile_cases quantize_fp8 [--rows 8192 --cols 8192] [--across] [--tiles] [--dtype f32]
+    python -m accera_b200.profile_cases embedding | embedding_grad [--table-rows 32000 --cols 4096 --indices 16384] [--dtype f16]
 
 Sizes default to cases whose inputs exceed the 126 MB L2 while holding well under a
 few GB on the device, so that a multi-pass profiler capture stays short.
@@ -43,6 +43,9 @@ def main() -> None:
     ap.add_argument("--b-row-major", action="store_true", help="gemm_bf16 / gemm_f16: B stored row-major (N contiguous)")
     ap.add_argument("--column-scales", action="store_true", help="gemm_fp8: a scale per column of B (the weight gradient) instead of per 128")
     ap.add_argument("--across", action="store_true", help="quantize_fp8: groups down the columns, transposed result")
+    ap.add_argument("--tiles", action="store_true", help="quantize_fp8: a scale per 128 x 128 instead of per 1 x 128")
+    ap.add_argument("--dtype", choices=["f32", "f16", "bf16"], default="bf16", help="quantize_fp8: type of x; embedding: of table and rows")
+    ap.add_argument("--block-major-scales", action="store_true", help="gemm_fp8: a block's scales of all rows and columns side by side")
     ap.add_argument("--option", action="append", default=[], metavar="NAME=VALUE",
                     help="a launch override for this run, e.g. gemm.group_n=16 (see accb_set_option)")
     a = ap.parse_args()
@@ -51,6 +54,7 @@ def main() -> None:
         rt.set_option(name, int(value))
     dev = torch.device("cuda:0")
     torch.manual_seed(0)
+    dtype = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[a.dtype]
     if a.case == "gemm_fp8":
         m, n, k = a.m or 8192, a.n or 8192, a.k or 8192
         A = torch.randn(m, k, device=dev).to(torch.float8_e4m3fn)
@@ -58,21 +62,23 @@ def main() -> None:
         blocks = -(-k // rt.FP8_BLOCK)
         sa = torch.rand(m, blocks, device=dev) + 0.5
         sb = (torch.rand(n if a.column_scales else -(-n // rt.FP8_BLOCK), blocks, device=dev) + 0.5).t()
+        if a.block_major_scales:
+            sa, sb = sa.t().contiguous().t(), sb.contiguous()
         C = torch.zeros(m, n, device=dev, dtype=torch.float32 if a.column_scales else torch.bfloat16)
         for _ in range(a.iters):
             rt.gemm_fp8(A, B, C, sa, sb, beta=0.0)
     elif a.case == "quantize_fp8":
-        x = torch.randn(a.rows, a.cols if a.cols != 4096 else 8192, device=dev).to(torch.bfloat16)
+        x = torch.randn(a.rows, a.cols if a.cols != 4096 else 8192, device=dev).to(dtype)
         x = x.t() if a.across else x
         q = torch.empty(x.shape, device=dev, dtype=torch.float8_e4m3fn)
-        s = torch.empty(x.shape[0], -(-x.shape[1] // rt.FP8_BLOCK), device=dev)
+        s = torch.empty(-(-x.shape[0] // rt.FP8_BLOCK) if a.tiles else x.shape[0], -(-x.shape[1] // rt.FP8_BLOCK), device=dev)
         for _ in range(a.iters):
             rt.quantize_fp8(x, q, s)
     elif a.case.startswith("embedding"):
-        T = (torch.randn(a.table_rows, a.cols, device=dev) * 0.02).to(torch.bfloat16)
+        T = (torch.randn(a.table_rows, a.cols, device=dev) * 0.02).to(dtype)
         u = torch.rand(a.indices, device=dev, dtype=torch.float64)          # word frequencies fall like one over the rank
         ids = (float(a.table_rows) ** u - 1).long().clamp_(0, a.table_rows - 1)
-        rows = torch.empty(a.indices, a.cols, device=dev, dtype=torch.bfloat16)
+        rows = torch.empty(a.indices, a.cols, device=dev, dtype=dtype)
         grad = torch.empty(a.table_rows, a.cols, device=dev)
         for _ in range(a.iters):
             rt.embedding(T, ids, rows, scale=64.0)

@@ -241,9 +241,10 @@ int accb_gather_rank2_dims(int64_t d0, int64_t d1, int64_t i0, int64_t i1, int32
  *
  * An id outside [0, vocab) is not dereferenced: its row is zero-filled (lookup) or left out (gradient) and
  * ACCB_ERR_INDEX is reported, from this call for host pointers and from the next accb_synchronize() for device
- * pointers.  Neither array may overlap the other.  A device-pointer accb_embedding_grad of more than
- * 2048 tokens takes its workspace (16 bytes a token and some partial sums) from a stream-ordered pool of the library, so calls on
- * several streams, and captured graphs, do not share it.
+ * pointers.  A call with nothing to write (no elements in a row, no tokens; for the gradient, no words) returns at once and looks
+ * at no id.  Neither array may overlap the other.  accb_embedding_grad of more than 2048 tokens takes its workspace (16 + dim / 4
+ * bytes a token: two lists, and partial sums of frequent words; 67 MB for 65536 tokens of 4096 columns) from a stream-ordered pool of
+ * the library, so calls on several streams, and captured graphs, do not share it; the pool keeps it until accb_release_workspace.
  * tokens is at most 2^30, vocab below 2^31 - 1, dim at most 2^20.
  */
 typedef struct accb_embedding_desc {
@@ -294,8 +295,8 @@ int accb_quantize_fp8(const accb_quantize_fp8_desc* desc, const void* x, void* q
  *   C <- epi(alpha * sum over blocks b of K:  sa[i, b] * sb[b, j] * (A[i, b] @ B[b, j])  +  beta * C + bias[j])
  *
  * a_type and b_type are ACCB_E4M3 or ACCB_E5M2, each its own; c_type is ACCB_F32, ACCB_F16 or ACCB_BF16; desc->compute is
- * ACCB_COMPUTE_AUTO, ACCB_COMPUTE_SIMT or ACCB_COMPUTE_TENSOR (which fails where ACCB_COMPUTE_AUTO would take the CUDA
- * cores); max_ctas > 0 takes the persistent kernel and bounds its grid (rounded up to an even number).  A block's products
+ * ACCB_COMPUTE_AUTO, ACCB_COMPUTE_SIMT or ACCB_COMPUTE_TENSOR (which fails where the tensor cores do not take an operand's
+ * layout; with K = 0 there is nothing to multiply, and every mode applies the epilogue to beta * C on the CUDA cores); max_ctas > 0 takes the persistent kernel and bounds its grid (rounded up to an even number).  A block's products
  * and the sum over blocks are accumulated in fp32; the product of a block's two scales is rounded to fp32 first.
  *
  * a_scales is ceil(M / a_block) x ceil(K / 128), b_scales ceil(K / 128) x ceil(N / b_block), a_block and b_block each
@@ -305,7 +306,7 @@ int accb_quantize_fp8(const accb_quantize_fp8_desc* desc, const void* x, void* q
  * the gradient of its weights.  C must not overlap anything that is read.
  *
  * Layouts: on the tensor cores each operand is contiguous along K or along its other direction; C has any strides.
- * Operands whose rows are not 16-byte aligned are copied into aligned rows first, and few-tile problems keep fp32 sums of
+ * Operands whose rows are not 16-byte aligned, or overlap, are copied into aligned rows first, and few-tile problems keep fp32 sums of
  * slices of K, both in stream-ordered temporaries of the library.  Host or device pointers as for accb_gemm.
  */
 typedef struct accb_fp8_scales {
@@ -394,7 +395,8 @@ const char* accb_version(void);
  *   "gemm_fp8.slices"        0 (choose) | 1 | 2 | 4 | 8   K slices of either
  *   "gemm_fp8.test_drop_scales"  0 | 1                self-test: the last scales of a tile (or of a CTA's slice of K) are never
  *                                                     signalled complete, with the same outcome as gemm.test_drop_commit
- *   "stream_kernels.pdl"     -1 (on) | 0 | 1          programmatic dependent launch of the reduce_mean, gather and range kernels
+ *   "stream_kernels.pdl"     -1 (on) | 0 | 1          programmatic dependent launch of the other kernels: reduce_mean, gather, range, embedding
+ *                                                     and its gradient, quantize_fp8, CUDA-core GEMMs, operand copies, sums of K slices
  *   "host_gemm.stage_chunks" 0 (16) | 1..256          row chunks of the staged host-pointer GEMM
  *   "reduce.rows_threads_per_output"  0 (choose) | 32 | 64 | 128 | 256   reduce_mean over contiguous segments
  */

@@ -634,3 +634,13 @@ def test_quantisation_of_infinities_nan_and_subnormals(block, across, src, to, m
     rt.synchronize()
     assert _same(s.cpu().double().numpy(), want[1])
     assert _same(q.cpu().double().numpy(), want[0])
+
+
+@pytest.mark.parametrize("compute", ["auto", "simt", "tensor"])
+def test_gemm_without_products_applies_the_epilogue_in_every_mode(compute):
+    f8 = lambda *shape: torch.zeros(*shape, device="cuda", dtype=torch.float8_e4m3fn)
+    old = torch.randn(6, 40, device="cuda")
+    C = old.clone()
+    rt.gemm_fp8(f8(6, 0), f8(0, 40), C, torch.zeros(6, 0, device="cuda"), torch.zeros(0, 1, device="cuda"), beta=-1.0, relu=True, compute=compute)
+    rt.synchronize()
+    assert torch.equal(C, torch.relu(-old))
