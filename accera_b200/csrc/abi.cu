@@ -47,13 +47,14 @@ thread_local cudaStream_t t_stream = nullptr;
 
 int fail(int code, const std::string& msg)
 {
+    // the runtime keeps a failed launch's error for this thread until it is asked: the next call must not find it
+    if (code == ACCB_ERR_CUDA) (void)cudaGetLastError();
     t_error = msg;
     return code;
 }
 
 int fail_cuda(const char* what, cudaError_t e)
 {
-    (void)cudaGetLastError();
     return fail(ACCB_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
